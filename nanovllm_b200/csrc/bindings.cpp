@@ -19,6 +19,11 @@ void prefill_attention_cuda(torch::Tensor q, torch::Tensor out, torch::Tensor cu
                             c10::optional<torch::Tensor> block_tables, c10::optional<torch::Tensor> kv_src,
                             int64_t nq, int64_t nkv, int64_t hd, double scale, double softcap, int64_t window,
                             bool causal, c10::optional<torch::Tensor> err);
+std::tuple<torch::Tensor, int64_t> shared_prefix_attention_cuda(
+    torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor prefix_blocks, int64_t prefix_len,
+    c10::optional<torch::Tensor> prefix_len_dev, torch::Tensor block_tables, torch::Tensor ctx_lens, double scale,
+    double softcap, int64_t window, c10::optional<torch::Tensor> cu_q, int64_t max_q, int64_t max_len,
+    c10::optional<torch::Tensor> out, torch::Tensor err);
 int64_t gemm_cuda(torch::Tensor x, torch::Tensor w, torch::Tensor out, int64_t act, c10::optional<torch::Tensor> workspace,
                   int64_t force_splits, c10::optional<torch::Tensor> err, bool partial_out);
 int64_t gemm_splits_for(int64_t M, int64_t N, int64_t K, int64_t act);
@@ -43,6 +48,9 @@ void shortconv_cuda(torch::Tensor proj, torch::Tensor weight, torch::Tensor cu, 
 void sample_cuda(torch::Tensor logits, torch::Tensor temps, torch::Tensor topk, torch::Tensor topp, torch::Tensor seeds,
                  torch::Tensor seq_ids, torch::Tensor steps, double softcap, torch::Tensor out,
                  c10::optional<torch::Tensor> ids);
+std::tuple<torch::Tensor, torch::Tensor, int64_t> verify_drafts_cuda(
+    torch::Tensor logits, torch::Tensor ids, torch::Tensor cu_q, int64_t max_q, torch::Tensor temps, torch::Tensor topk,
+    torch::Tensor topp, torch::Tensor uniforms, c10::optional<torch::Tensor> probs, double softcap, torch::Tensor err);
 void rms_norm_post_add_cuda(torch::Tensor x, torch::Tensor residual, c10::optional<torch::Tensor> weight, double eps,
                             int64_t mode, double post_scale);
 void ple_combine_cuda(torch::Tensor out, torch::Tensor proj, torch::Tensor tok, torch::Tensor weight, double eps,
@@ -74,6 +82,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qk_norm_rope_store", &qk_norm_rope_store_cuda);
   m.def("paged_decode", &paged_decode_cuda);
   m.def("prefill_attention", &prefill_attention_cuda);
+  m.def("shared_prefix_attention", &shared_prefix_attention_cuda);
   m.def("gemm", &gemm_cuda);
   m.def("gemm_splits_for", &gemm_splits_for);
   m.def("gemm_sp", &gemm_sp_cuda);
@@ -94,6 +103,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gather_rows", &gather_rows_cuda);
   m.def("mean_pool_l2", &mean_pool_l2_cuda);
   m.def("sample", &sample_cuda);
+  m.def("verify_drafts", &verify_drafts_cuda);
   m.def("shortconv", &shortconv_cuda);
   m.def("rms_norm_post_add", &rms_norm_post_add_cuda);
   m.def("ple_combine", &ple_combine_cuda);

@@ -5,7 +5,7 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <torch/extension.h>
+#include <c10/util/Exception.h>
 
 #include <array>
 #include <cstring>

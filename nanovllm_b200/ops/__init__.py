@@ -318,6 +318,56 @@ def prefill_attention(q, cu_q, cu_k, max_q, nq, nkv, hd, scale, softcap=0.0, win
     return out
 
 
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise RuntimeError(message)
+
+
+def shared_prefix_attention(q, k_cache, v_cache, prefix_blocks, prefix_len, block_tables, ctx_lens, scale, softcap=0.0,
+                            window=0, cu_q=None, max_q=1, max_len=None, out=None):
+    """Paged attention of sequences that begin with the same ``prefix_len`` tokens, read once for all of them.
+
+    q [T, nq, hd]: one query token per sequence, or with ``cu_q`` (int32 [B + 1]) rows cu_q[b] .. cu_q[b + 1] - 1 of
+    sequence b, at most ``max_q`` each; they are its last tokens, already stored in the caches.  ``ctx_lens`` (int32
+    [B]) counts all keys of a sequence, those tokens included.  Key j is read from page ``prefix_blocks[j // block]``
+    while j < ``prefix_len`` and from ``block_tables[b, j // block]`` after that: the tables count pages from the
+    sequence's first token, as everywhere in the engine, and their entries for whole shared pages are not read.
+    ``prefix_len`` is an int or, for calls in a CUDA graph, one int32 on the device.  A sequence may be shorter than
+    the prefix; with no key to see (context 0) its rows are zero.  ``max_len`` bounds ``ctx_lens`` (default: what
+    the tables hold).  Rows behind the last sequence are not written.
+
+    Values in the caches at keys that no row sees may be anything.  A context beyond ``max_len`` or its table, a page
+    number outside the caches or a sequence of more than ``max_q`` tokens is reported by ``check_device_errors``; the
+    rows of that sequence (for a bad prefix: all rows) are then undefined."""
+    if max_len is None:
+        max_len = max(block_tables.shape[1], prefix_blocks.shape[0]) * k_cache.shape[2]
+    on_device = isinstance(prefix_len, torch.Tensor)
+    if not q.is_cuda:
+        T, nq, hd = q.shape
+        B = ctx_lens.shape[0]
+        _require(k_cache.shape == v_cache.shape and k_cache.dim() == 4 and k_cache.shape[3] == hd,
+                 "caches must both be [num_blocks, nkv, block, hd]")
+        _require(nq % k_cache.shape[1] == 0, "query heads must be a multiple of the KV heads")
+        _require(k_cache.shape[2] % 64 == 0, "block size must be a multiple of 64")
+        _require(prefix_blocks.dim() == 1 and block_tables.dim() == 2 and block_tables.shape[0] == B,
+                 "prefix_blocks must be [pages], block_tables one row per sequence")
+        _require(all(t.dtype == torch.int32 for t in (prefix_blocks, block_tables, ctx_lens)), "int32 metadata")
+        _require(0 <= int(prefix_len) <= prefix_blocks.numel() * k_cache.shape[2],
+                 "prefix_len must lie between 0 and the keys of prefix_blocks")
+        _require(T == B if cu_q is None else cu_q.numel() == B + 1,
+                 "without cu_q there is one query token per sequence, with it one entry more than sequences")
+        _require(max_q >= 1 and max_len >= 0 and window >= 0 and softcap >= 0.0,
+                 "max_q must be at least 1; max_len, window and softcap not negative")
+        _require(out is None or (out.shape == q.shape and out.dtype == q.dtype), "out must be of the shape of q")
+        return ref.shared_prefix_attention(q, k_cache, v_cache, prefix_blocks, prefix_len, block_tables, ctx_lens,
+                                           scale, softcap, window, cu_q, out)
+    out, launches = _cuda_ext().shared_prefix_attention(
+        q, k_cache, v_cache, prefix_blocks, 0 if on_device else prefix_len, prefix_len if on_device else None,
+        block_tables, ctx_lens, scale, softcap, window, cu_q, max_q, max_len, out, error_word(q.device))
+    add_launches(launches)
+    return out
+
+
 # ------------------------------------------------------------------------------------------------ linear
 def library_gemm() -> bool:
     """``NVB_BASELINE=1``: every projection runs as a cuBLAS GEMM (torch.matmul) with the activation as a
@@ -502,6 +552,45 @@ def sample(logits, temps, top_ks, top_ps, seeds, seq_ids, steps, softcap: float 
     _cuda_ext().sample(logits, temps, top_ks, top_ps, seeds, seq_ids, steps, float(softcap), out, ids)
     add_launches(1)
     return out
+
+
+def verify_drafts(logits, ids, cu_q, max_q, temps, top_ks, top_ps, uniforms, draft_probs=None, softcap: float = 0.0
+                  ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stay, and the token after them (speculative sampling), from given uniforms.
+
+    Rows cu_q[b] .. cu_q[b + 1] - 1 of ``logits`` (bf16 or fp32 [R, V]) are sequence b's target logits for the tokens
+    after ``ids`` (int64 [R], the step's input tokens): row r is held against the draft ids[r + 1], the sequence's last
+    row scores what follows the last draft.  ``temps``, ``top_ks``, ``top_ps`` ([B]) cut the target's distribution p as
+    in ``sample`` (top_k 1: greedy).  ``draft_probs`` (fp32, one row per draft, in order): the distributions q that the
+    drafts were drawn from; without it the drafts were certain (q = 1 at the draft), as looked-up drafts are.
+
+    Draft d of row r is accepted while uniforms[r] * q[d] < p[d].  The token after the accepted drafts is drawn from
+    max(0, p - q) of the refused row (without q: p without d), or from p of the last row when none was refused, by the
+    inverse of its cumulated sum in token order with the uniform of the sequence's last row (fp32 or fp64, [0, 1)), so
+    the emitted tokens are distributed as tokens sampled one by one.  A draft outside the vocabulary is refused.
+
+    Returns (tokens int64 [B, max_q]: accepted drafts, the drawn token, then -1; counts int32 [B]: tokens emitted, 0
+    for a sequence without rows).  A sequence of more than ``max_q`` rows is reported by ``check_device_errors`` and
+    emits nothing."""
+    if not logits.is_cuda:
+        R, V = logits.shape
+        B = cu_q.numel() - 1
+        _require(logits.dtype in (torch.bfloat16, torch.float32), "logits must be bf16 or fp32 [rows, vocabulary]")
+        _require(1 <= V <= 1 << 20, "the vocabulary must have 1 to 1048576 tokens")
+        for t, dtypes, n, name in ((cu_q, (torch.int32,), B + 1, "cu_q"), (ids, (torch.int64,), R, "ids"),
+                                   (temps, (torch.float32,), B, "temps"), (top_ks, (torch.int32,), B, "top_ks"),
+                                   (top_ps, (torch.float32,), B, "top_ps"),
+                                   (uniforms, (torch.float32, torch.float64), R, "uniforms")):
+            _require(t.dtype in dtypes and t.dim() == 1 and t.numel() == n, f"{name} must be a vector of {n}")
+        _require(draft_probs is None or (draft_probs.dtype == torch.float32 and draft_probs.dim() == 2
+                                         and draft_probs.shape[1] == V),
+                 "draft_probs must be fp32 [drafts, vocabulary]")
+        _require(max_q >= 1 and softcap >= 0.0, "max_q must be at least 1, softcap not negative")
+        return ref.verify_drafts(logits, ids, cu_q, max_q, temps, top_ks, top_ps, uniforms, draft_probs, softcap)
+    tokens, counts, launches = _cuda_ext().verify_drafts(logits, ids, cu_q, max_q, temps, top_ks, top_ps, uniforms,
+                                                         draft_probs, softcap, error_word(logits.device))
+    add_launches(launches)
+    return tokens, counts
 
 
 def shortconv(proj, weight, cu, rows, fresh, state, state_off: int):

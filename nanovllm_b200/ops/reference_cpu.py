@@ -185,6 +185,36 @@ def prefill_attention(q: torch.Tensor, cu_q, cu_k, nq, nkv, hd, scale, softcap=0
     return out
 
 
+def shared_prefix_attention(q, k_cache, v_cache, prefix_blocks, prefix_len, block_tables, ctx_lens, scale, softcap=0.0,
+                            window=0, cu_q=None, out=None):
+    """q [T, nq, hd]; sequence b's keys are the first ``prefix_len`` tokens of the pages ``prefix_blocks``, then its
+    own pages (``block_tables`` counts pages from the sequence's first token).  Rows behind cu_q[-1] stay as they
+    were in ``out``."""
+    T, nq, D = q.shape
+    G = nq // k_cache.shape[1]
+    P, bs = int(prefix_len), k_cache.shape[2]
+    out = torch.zeros_like(q) if out is None else out
+    for b in range(len(ctx_lens)):
+        n = int(ctx_lens[b])
+        t0, t1 = (b, b + 1) if cu_q is None else (int(cu_q[b]), int(cu_q[b + 1]))
+        if t1 <= t0:
+            continue
+        shared = min(P, n)
+        k = torch.empty(n, k_cache.shape[1], D, dtype=k_cache.dtype)
+        v = torch.empty_like(k)
+        for dst, cache in ((k, k_cache), (v, v_cache)):
+            if shared:
+                dst[:shared] = _gather_paged(cache, prefix_blocks, shared)
+            if n > shared:
+                first = shared // bs
+                own = _gather_paged(cache, block_tables[b, first:], n - first * bs)
+                dst[shared:] = own[shared - first * bs:]
+        qpos = torch.arange(n - (t1 - t0), n)
+        out[t0:t1] = _attend(q[t0:t1], k.repeat_interleave(G, dim=1), v.repeat_interleave(G, dim=1), qpos, True,
+                             window, scale, softcap).to(q.dtype)
+    return out
+
+
 def interleave_gate_up(gate_up: torch.Tensor, block: int = 128) -> torch.Tensor:
     """[gate(I); up(I)] rows -> blocks [gate_b; up_b] of ``block`` rows each (the layout of the fused kernels)."""
     I = gate_up.shape[0] // 2
@@ -310,6 +340,70 @@ def sample(logits: torch.Tensor, temps, top_ks, top_ps, seeds, seq_ids, steps, s
         score = p[idxs].double().numpy() / np.maximum(1e-10, g)
         out[r] = int(gidx[int(np.argmax(score))])
     return out
+
+
+def target_probs(logits: torch.Tensor, temp: float, top_k: int, top_p: float, softcap: float = 0.0) -> torch.Tensor:
+    """One row's probabilities (64 bits) after soft-cap, temperature, top-k and top-p; NaN logits count as -inf.  All
+    zeros when no logit is above -inf."""
+    raw = torch.nan_to_num(logits.double(), nan=float("-inf"), posinf=float("inf"), neginf=float("-inf"))
+    x = softcap * torch.tanh(raw / softcap) if softcap > 0 else raw
+    V, m = x.numel(), float(raw.max())
+    if m == float("-inf"):
+        return torch.zeros_like(x)
+    order = torch.sort(-raw, stable=True).indices  # value descending, index ascending on ties
+    top = raw == m
+    w = torch.where(top, torch.ones_like(x), torch.exp((x - x[order[0]]) / temp))
+    w = torch.where((raw == float("-inf")) & (softcap <= 0), torch.zeros_like(w), w)
+    if top_k == 1:  # whatever the temperature is
+        w = top.double()
+    n = V if top_k <= 0 or top_k > V else top_k
+    if top_p < 1.0:
+        c = torch.cumsum(w[order[:n]], 0)
+        n = max(1, int((c - w[order[:n]] < top_p * c[-1]).sum()))
+    p = torch.zeros_like(w)
+    p[order[:n]] = w[order[:n]]
+    return p / p.sum()
+
+
+def verify_drafts(logits, ids, cu_q, max_q, temps, top_ks, top_ps, uniforms, draft_probs=None, softcap=0.0):
+    """Speculative sampling row by row: accept ids[r + 1] while u_r * q_d < p_d; at the first refusal draw from
+    max(0, p - q), else from p of the last row, by the cumulated sum in token order and the last row's uniform."""
+    B, V = len(cu_q) - 1, logits.shape[1]
+    tokens = torch.full((B, max_q), -1, dtype=torch.long)
+    counts = torch.zeros(B, dtype=torch.int32)
+    drow = 0
+    for b in range(B):
+        r0, n, acc = int(cu_q[b]), int(cu_q[b + 1]) - int(cu_q[b]), 0
+        if n <= 0:
+            continue
+        while True:
+            r = r0 + acc
+            p = target_probs(logits[r], float(temps[b]), int(top_ks[b]), float(top_ps[b]), softcap)
+            if acc == n - 1:
+                break
+            d = int(ids[r + 1])
+            known = 0 <= d < V
+            q = None if draft_probs is None else draft_probs[drow + acc].double()
+            if known and float(uniforms[r]) * (1.0 if q is None else float(q[d])) < float(p[d]):
+                tokens[b, acc] = d
+                acc += 1
+                continue
+            left = p.clone()
+            if q is not None:
+                left = torch.clamp(p - q, min=0.0)
+            elif known:
+                left[d] = 0.0
+            p = left if float(left.sum()) > 0 else p
+            break
+        c = torch.cumsum(p, 0)
+        if float(c[-1]) > 0:
+            u = min(max(float(uniforms[r0 + n - 1]), 0.0), 1.0 - 2.0 ** -52)
+            tokens[b, acc] = int(torch.nonzero(c > u * c[-1])[0])
+        else:
+            tokens[b, acc] = 0
+        counts[b] = acc + 1
+        drow += n - 1
+    return tokens, counts
 
 
 def shortconv(proj: torch.Tensor, weight: torch.Tensor, cu: torch.Tensor, rows: torch.Tensor, fresh: torch.Tensor,
