@@ -11,6 +11,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -135,6 +136,468 @@ __global__ void __launch_bounds__(128) sp_generic_kernel(SpArgs a, const bf16* _
     if (lane + 32 * i < a.hd) a.out[t * a.o_tok + h * a.o_head + lane + 32 * i] = __float2bfloat16(acc[i] * inv);
 }
 
+// ------------------------------------------------------------------------------------------------ split kernels
+// o = sum_i w_i O_i / sum_i w_i with w_i = 2^(lse_i - max lse): every part of the keys (a range of the prefix or of a
+// sequence's own keys) is reduced by one CTA to a normalised fp32 row O_i and its log2-sum-exp, and a last kernel
+// joins them.  Parts are written by every CTA, also by one whose range is empty (lse -inf), so nothing needs clearing.
+constexpr int KT = 64;       // keys per tile
+constexpr int kRows = 64;    // query rows (token, head of the group) per CTA of the mma.sync kernel
+constexpr int kCuSmem = 1024;  // sequences whose cu_q fits the shared copy
+
+struct SpPlan {
+  int n_pre, pre_tiles, pre_row_tiles;  // prefix: key splits, tiles per split, row tiles
+  int n_own, own_tiles, own_row_tiles;  // own keys: the same, per sequence
+  float* part_o;                        // [T, nq, n_pre + n_own, hd]
+  float* part_lse;                      // [T, nq, n_pre + n_own]
+};
+
+NV_DEVICE int sp_page(const SpArgs& a, const int* pages, int key) {
+  const int blk = pages[key / a.block_size];
+  if (blk < 0 || blk >= a.num_blocks) {
+    nvb::record_error(a.err, nvb::kErrBadArgument);
+    return 0;
+  }
+  return blk;
+}
+
+// cu_q in shared memory (global beyond kCuSmem sequences): the search for a row's sequence is then free of
+// dependent global loads.
+NV_DEVICE const int* stage_cu(const SpArgs& a, int* sh, int threads) {
+  if (a.cu_q == nullptr || a.B >= kCuSmem) return a.cu_q;
+  for (int i = threadIdx.x; i <= a.B; i += threads) sh[i] = a.cu_q[i];
+  return sh;
+}
+
+// Position of query token t (-1: it sees no key, also for rows behind the last sequence or of a refused one).
+NV_DEVICE int row_position(const SpArgs& a, const int* cu, int t, int P) {
+  if (t >= a.T) return -1;
+  int b = t, i = 0, n = 1;
+  if (cu != nullptr) {
+    b = seq_of(cu, a.B, t);
+    const int lo = cu[b], hi = cu[b + 1];
+    i = t - lo, n = hi - lo;
+    if (lo < 0 || hi > a.T || t < lo || t >= hi || n > a.max_q) return -1;
+  }
+  const int ctx = a.ctx_lens[b];
+  return a.ctx_ok(ctx, P) ? ctx - n + i : -1;
+}
+
+// One part: rows [row0, row0 + rows) of a (token, head) list against tiles [t0, t1) of the keys [klo, kend).
+struct SpPart {
+  int tok0, row0, rows;  // row r: token tok0 + (row0 + r) / G, head kvh * G + (row0 + r) % G
+  int kvh, slot;
+  int klo, kend, t0, t1;
+  const int* pages;
+};
+
+// Four warps: RG groups of 16 rows times 4 / RG groups of 16 * RG keys of each tile.  S and O stay in registers
+// (mma.sync m16n8k16), Q in registers up to head dim 128.
+template <int HD, int STAGES, int RG>
+__device__ void sp_part_mma(const SpArgs& a, const SpPlan& pl, const SpPart& p, const CUtensorMap* kmap,
+                            const CUtensorMap* vmap, uint8_t* ring, uint64_t* bars, bf16* qs, const int* row_pos,
+                            volatile int* abort_flag) {
+  constexpr int TILE = KT * HD * 2;
+  constexpr int KW = 16 * RG;  // keys of a warp
+  constexpr int NB = KW / 8;
+  constexpr int QP = HD + 8;
+  constexpr bool kQRegs = HD <= 128;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
+  const int rg = warp % RG, key0 = (warp / RG) * KW;
+  const int G = a.nq / a.nkv, nt = p.t1 - p.t0;
+  auto issue = [&](int i) {
+    const int st = i % STAGES, tok = (p.t0 + i) * KT;
+    const int row = (sp_page(a, p.pages, tok) * a.nkv + p.kvh) * a.block_size + tok % a.block_size;
+    uint8_t* kd = ring + st * 2 * TILE;
+    nvb::mbar_arrive_expect_tx(&bars[st], 2 * TILE);
+#pragma unroll
+    for (int j = 0; j < HD / 64; ++j) {
+      nvb::tma_load_2d(kd + j * KT * 128, kmap, &bars[st], j * 64, row);
+      nvb::tma_load_2d(kd + TILE + j * KT * 128, vmap, &bars[st], j * 64, row);
+    }
+  };
+  if (tid == 0)
+    for (int i = 0; i < STAGES && i < nt; ++i) issue(i);
+  auto q_row = [&](int r) {
+    const int f = p.row0 + r;
+    return a.q + (long)(p.tok0 + f / G) * a.q_tok + (long)(p.kvh * G + f % G) * a.q_head;
+  };
+  uint32_t qf[kQRegs ? HD / 16 : 1][4];
+  if constexpr (kQRegs) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = rg * 16 + g + h * 8;
+      const bf16* src = r < p.rows ? q_row(r) : nullptr;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        qf[kk][h] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 2 * c4) : 0u;
+        qf[kk][h + 2] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + 8 + 2 * c4) : 0u;
+      }
+    }
+  } else {
+    for (int idx = tid; idx < 16 * RG * (HD / 8); idx += 128) {
+      const int r = idx / (HD / 8), c = idx % (HD / 8);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < p.rows) v = *reinterpret_cast<const uint4*>(q_row(r) + c * 8);
+      *reinterpret_cast<uint4*>(qs + r * QP + c * 8) = v;
+    }
+    __syncthreads();
+  }
+  int rpos[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = rg * 16 + g + h * 8;
+    rpos[h] = r < p.rows ? row_pos[r] : -1;
+  }
+  const int win = a.window > 0 ? a.window : 0x40000000;
+  float o[HD / 8][4];
+#pragma unroll
+  for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  const float sl2 = a.scale * kLog2e;
+  const int mi = lane >> 3, lr = lane & 7;
+  bool aborted = false;
+  for (int i = 0; i < nt; ++i) {
+    const int st = i % STAGES;
+    const bool ok = nvb::mbar_wait(&bars[st], (uint32_t)((i / STAGES) & 1), a.err, abort_flag);
+    if (__syncthreads_or(!ok)) { aborted = true; break; }
+    uint8_t* vt = ring + st * 2 * TILE + TILE;
+    const uint32_t kb = nvb::smem_u32(ring + st * 2 * TILE), vb = kb + TILE;
+    const int tok0 = (p.t0 + i) * KT;
+    if (tok0 < p.klo || tok0 + KT > p.kend) {
+      // keys outside the part may hold anything: their weight is 0, and 0 * NaN must not reach the sum
+      const int lo = max(0, p.klo - tok0), hi = min(KT, p.kend - tok0);
+      for (int idx = tid; idx < KT * (HD / 8); idx += 128) {
+        const int r = idx / (HD / 8), c = idx % (HD / 8);
+        if (r < lo || r >= hi)
+          *reinterpret_cast<uint4*>(vt + (c >> 3) * (KT * 128) + nvb::swz128(r, c & 7)) = make_uint4(0, 0, 0, 0);
+      }
+      nvb::fence_proxy_async();  // before a later TMA copy into the same stage
+      __syncthreads();
+    }
+    if (rg * 16 < p.rows) {
+      float s[NB][4];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        uint32_t af[4];
+        if constexpr (kQRegs) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) af[e] = qf[kk][e];
+        } else {
+          nvb::ldmatrix_x4(af[0], af[1], af[2], af[3],
+                           nvb::smem_u32(qs) + ((rg * 16 + (lane & 15)) * QP + kk * 16 + (lane >> 4) * 8) * 2);
+        }
+#pragma unroll
+        for (int np = 0; np < NB / 2; ++np) {
+          const int key = key0 + np * 16 + lr + (mi >> 1) * 8, dim = kk * 16 + (mi & 1) * 8;
+          uint32_t b0, b1, b2, b3;
+          nvb::ldmatrix_x4(b0, b1, b2, b3, kb + (uint32_t)(dim >> 6) * (KT * 128) + nvb::swz128(key, (dim & 63) >> 3));
+          nvb::mma_bf16_16816(s[2 * np], af, b0, b1);
+          nvb::mma_bf16_16816(s[2 * np + 1], af, b2, b3);
+        }
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = e >> 1, key = tok0 + key0 + n * 8 + 2 * c4 + (e & 1);
+          float x = a.softcap > 0.f ? sp_cap(s[n][e] * a.scale, a.softcap) * kLog2e : s[n][e] * sl2;
+          if (key > rpos[h] || key < p.klo || key >= p.kend || key <= rpos[h] - win) x = -INFINITY;
+          s[n][e] = x;
+          mx[h] = fmaxf(mx[h], x);
+        }
+      float corr[2], rs[2] = {0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        const float nm = fmaxf(m_run[h], mx[h]);
+        corr[h] = nm == -INFINITY ? 1.f : exp2f(m_run[h] - nm);
+        m_run[h] = nm;
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = e >> 1;
+          const float w = m_run[h] == -INFINITY ? 0.f : exp2f(s[n][e] - m_run[h]);
+          s[n][e] = w;
+          rs[h] += w;
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) l_run[h] = l_run[h] * corr[h] + rs[h];
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) {
+        o[d][0] *= corr[0];
+        o[d][1] *= corr[0];
+        o[d][2] *= corr[1];
+        o[d][3] *= corr[1];
+      }
+      // the weights are rounded to bf16 for the product (2^-8 of each, as everywhere in this engine); the
+      // denominator sums them unrounded
+#pragma unroll
+      for (int ks = 0; ks < KW / 16; ++ks) {
+        const uint32_t pa[4] = {nvb::pack_bf16x2(s[2 * ks][0], s[2 * ks][1]), nvb::pack_bf16x2(s[2 * ks][2], s[2 * ks][3]),
+                                nvb::pack_bf16x2(s[2 * ks + 1][0], s[2 * ks + 1][1]),
+                                nvb::pack_bf16x2(s[2 * ks + 1][2], s[2 * ks + 1][3])};
+#pragma unroll
+        for (int dp = 0; dp < HD / 16; ++dp) {
+          const int key = key0 + ks * 16 + lr + (mi & 1) * 8, dim = dp * 16 + (mi >> 1) * 8;
+          uint32_t b0, b1, b2, b3;
+          nvb::ldmatrix_x4_trans(b0, b1, b2, b3,
+                                 vb + (uint32_t)(dim >> 6) * (KT * 128) + nvb::swz128(key, (dim & 63) >> 3));
+          nvb::mma_bf16_16816(o[2 * dp], pa, b0, b1);
+          nvb::mma_bf16_16816(o[2 * dp + 1], pa, b2, b3);
+        }
+      }
+    }
+    __syncthreads();
+    if (tid == 0 && i + STAGES < nt) issue(i + STAGES);
+  }
+  if (aborted) {  // reported in the error word; drain the copies still in flight (bounded)
+    if (tid == 0)
+      for (int s = 0; s < STAGES; ++s) nvb::mbar_wait(&bars[s], 0, nullptr, nullptr);
+    return;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
+    l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+  }
+  const int NS = pl.n_pre + pl.n_own;
+  auto slot_of = [&](int r) {
+    const int f = p.row0 + r;
+    return ((long)(p.tok0 + f / G) * a.nq + p.kvh * G + f % G) * NS + p.slot;
+  };
+  if constexpr (RG == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = rg * 16 + g + h * 8;
+      if (r >= p.rows) continue;
+      const long slot = slot_of(r);
+      const float inv = l_run[h] > 0.f ? 1.f / l_run[h] : 0.f;
+      float* dst = pl.part_o + slot * HD;
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+        *reinterpret_cast<float2*>(dst + d * 8 + 2 * c4) = make_float2(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+      if (c4 == 0) pl.part_lse[slot] = l_run[h] > 0.f ? m_run[h] + log2f(l_run[h]) : -INFINITY;
+    }
+  } else {
+    // join the key groups of a row group through shared memory (the ring is free: every tile was waited for)
+    float* comb = reinterpret_cast<float*>(ring);  // [4 warps][16][HD]
+    float* cm = comb + 4 * 16 * HD;                // [4][16]
+    float* cl = cm + 64;
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(comb + (warp * 16 + g + h * 8) * HD + d * 8 + 2 * c4) =
+            make_float2(o[d][2 * h], o[d][2 * h + 1]);
+    if (c4 == 0)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        cm[warp * 16 + g + h * 8] = m_run[h];
+        cl[warp * 16 + g + h * 8] = l_run[h];
+      }
+    __syncthreads();
+    for (int idx = tid; idx < p.rows * (HD / 4); idx += 128) {
+      const int r = idx / (HD / 4), d = (idx % (HD / 4)) * 4;
+      const int w0 = r >> 4, rr = r & 15;  // warps w0, w0 + RG, ... hold the row
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4 / RG; ++w) M = fmaxf(M, cm[(w0 + w * RG) * 16 + rr]);
+      float L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (M != -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < 4 / RG; ++w) {
+          const int at = (w0 + w * RG) * 16 + rr;
+          const float f = exp2f(cm[at] - M);
+          const float4 v = *reinterpret_cast<const float4*>(comb + at * HD + d);
+          L += cl[at] * f;
+          acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+        }
+      }
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const long slot = slot_of(r);
+      *reinterpret_cast<float4*>(pl.part_o + slot * HD + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (d == 0) pl.part_lse[slot] = L > 0.f ? M + log2f(L) : -INFINITY;
+    }
+  }
+}
+
+template <int HD, int STAGES>
+constexpr size_t sp_mma_smem() {
+  return 1024 + STAGES * 2 * KT * HD * 2 + (HD <= 128 ? 0 : kRows * (HD + 8) * 2) + 64;
+}
+
+// Grid: the parts of the prefix (split fastest, then KV head, then row tile), then those of the sequences' own keys
+// (split, KV head, row tile, sequence).  K/V tiles of 64 keys come through TMA into a ring of STAGES; bound by the
+// bytes of the cache as long as a tile serves few rows.
+template <int HD, int STAGES>
+__global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                     const __grid_constant__ CUtensorMap vmap, SpArgs a, SpPlan pl) {
+  nvb::pdl_wait();
+  nvb::pdl_trigger();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  bf16* qs = reinterpret_cast<bf16*>(ring + STAGES * 2 * KT * HD * 2);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(qs) + (HD <= 128 ? 0 : kRows * (HD + 8) * 2));
+  __shared__ int abort_flag, cu_sh[kCuSmem + 1], row_pos[kRows], pos_lo, pos_hi;
+  const int tid = threadIdx.x;
+  const int G = a.nq / a.nkv, P = a.prefix_len();
+  const bool p_ok = a.prefix_ok(P);
+  SpPart p{};
+  int bid = blockIdx.x;
+  const int n_prefix = pl.n_pre * a.nkv * pl.pre_row_tiles;
+  const bool is_prefix = bid < n_prefix;
+  if (tid == 0) {
+    abort_flag = 0;
+    pos_lo = 0x7fffffff;
+    pos_hi = -1;
+    for (int s = 0; s < STAGES; ++s) nvb::mbar_init(&bars[s], 1);
+    nvb::fence_mbar_init();
+    nvb::tma_prefetch_desc(&kmap);
+    nvb::tma_prefetch_desc(&vmap);
+  }
+  if (is_prefix) {
+    const int split = bid % pl.n_pre;
+    bid /= pl.n_pre;
+    p.kvh = bid % a.nkv;
+    p.row0 = (bid / a.nkv) * kRows;
+    p.rows = min(kRows, a.T * G - p.row0);
+    p.slot = split;
+    p.kend = p_ok ? P : 0;
+    p.t0 = split * pl.pre_tiles;
+    p.t1 = p.t0 + pl.pre_tiles;
+    p.pages = a.prefix_blocks;
+    const int* cu = stage_cu(a, cu_sh, 128);
+    __syncthreads();
+    if (tid < kRows && tid < p.rows) {
+      const int pos = row_position(a, cu, (p.row0 + tid) / G, P);
+      row_pos[tid] = pos;
+      if (pos >= 0) {
+        atomicMin(&pos_lo, pos);
+        atomicMax(&pos_hi, pos);
+      }
+    }
+  } else {
+    bid -= n_prefix;
+    const int split = bid % pl.n_own;
+    bid /= pl.n_own;
+    p.kvh = bid % a.nkv;
+    bid /= a.nkv;
+    const int b = bid / pl.own_row_tiles;
+    const int2 tk = a.tokens(b);
+    const int ctx = a.ctx_lens[b], n = tk.y - tk.x;
+    if (n < 0 || !p_ok || !a.ctx_ok(ctx, P)) {  // reported; the sequence's rows are undefined
+      if (tid == 0) nvb::record_error(a.err, nvb::kErrBadArgument);
+      return;
+    }
+    p.tok0 = tk.x;
+    p.row0 = (bid % pl.own_row_tiles) * kRows;
+    p.rows = min(kRows, n * G - p.row0);
+    if (p.rows <= 0) return;
+    p.slot = pl.n_pre + split;
+    p.klo = P;
+    p.kend = ctx;
+    p.t0 = P / KT + split * pl.own_tiles;
+    p.t1 = p.t0 + pl.own_tiles;
+    p.pages = a.block_tables + b * a.bt_stride;
+    __syncthreads();
+    if (tid < p.rows) {
+      const int pos = ctx - n + (p.row0 + tid) / G;
+      row_pos[tid] = pos;
+      if (tid == 0) pos_lo = pos;
+      if (tid == p.rows - 1) pos_hi = pos;
+    }
+  }
+  __syncthreads();
+  if (is_prefix && !p_ok && tid == 0) nvb::record_error(a.err, nvb::kErrBadArgument);
+  // only tiles that some row sees
+  p.kend = min(p.kend, pos_hi + 1);
+  p.t1 = p.kend > p.klo ? min(p.t1, (p.kend + KT - 1) / KT) : p.t0;
+  if (a.window > 0 && pos_lo != 0x7fffffff) p.t0 = max(p.t0, max(0, pos_lo - a.window + 1) / KT);
+  if (p.t0 >= p.t1) {
+    const int NS = pl.n_pre + pl.n_own;
+    if (tid < p.rows) {
+      const int f = p.row0 + tid;
+      pl.part_lse[((long)(p.tok0 + f / G) * a.nq + p.kvh * G + f % G) * NS + p.slot] = -INFINITY;
+    }
+    return;
+  }
+  if (p.rows <= 16) sp_part_mma<HD, STAGES, 1>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
+  else if (p.rows <= 32) sp_part_mma<HD, STAGES, 2>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
+  else sp_part_mma<HD, STAGES, 4>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
+}
+
+// One warp per (token, head): joins the parts.
+template <int HD>
+__global__ void __launch_bounds__(128) sp_join_kernel(SpArgs a, SpPlan pl) {
+  nvb::pdl_wait();
+  nvb::pdl_trigger();
+  const long row = ((long)blockIdx.x * 128 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (row >= (long)a.T * a.nq) return;
+  const int t = (int)(row / a.nq), h = (int)(row % a.nq);
+  if (a.cu_q != nullptr && (t < a.cu_q[0] || t >= a.cu_q[a.B])) return;  // a row behind the last sequence
+  const int NS = pl.n_pre + pl.n_own;
+  const float* lse = pl.part_lse + row * NS;
+  const float* po = pl.part_o + row * NS * HD;
+  float M = -INFINITY;
+  for (int s = lane; s < NS; s += 32) M = fmaxf(M, lse[s]);
+  M = nvb::warp_max(M);
+  constexpr int PER = HD / 32;  // 2, 4 or 8 values per lane
+  float acc[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+  float den = 0.f;
+  if (M != -INFINITY)
+    for (int s0 = 0; s0 < NS; s0 += 32) {
+      const float w = s0 + lane < NS ? exp2f(lse[s0 + lane] - M) : 0.f;
+      for (unsigned left = __ballot_sync(0xffffffffu, w > 0.f); left != 0; left &= left - 1) {
+        const int s = __ffs(left) - 1;
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+        den += ws;
+        const float* src = po + (long)(s0 + s) * HD + lane * PER;
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) {
+          const float2 v = *reinterpret_cast<const float2*>(src + i);
+          acc[i] += ws * v.x;
+          acc[i + 1] += ws * v.y;
+        }
+      }
+    }
+  const float inv = den > 0.f ? 1.f / den : 0.f;
+  bf16* dst = a.out + t * a.o_tok + h * a.o_head + lane * PER;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2)
+    *reinterpret_cast<uint32_t*>(dst + i) = nvb::pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+}
+
+template <int HD, int STAGES>
+void launch_split(const SpArgs& a, const SpPlan& pl, const void* kc, const void* vc, cudaStream_t stream) {
+  const uint64_t rows = (uint64_t)a.num_blocks * a.nkv * a.block_size;
+  const CUtensorMap km = nvb::make_tmap_2d_bf16(kc, rows, HD, HD, KT);
+  const CUtensorMap vm = nvb::make_tmap_2d_bf16(vc, rows, HD, HD, KT);
+  auto kern = sp_mma_kernel<HD, STAGES>;
+  constexpr size_t sm = sp_mma_smem<HD, STAGES>();
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+  const unsigned grid = (unsigned)(pl.n_pre * a.nkv * pl.pre_row_tiles + pl.n_own * a.nkv * pl.own_row_tiles * a.B);
+  if (grid > 0) C10_CUDA_CHECK(nvb::launch(kern, dim3(grid), dim3(128), sm, stream, km, vm, a, pl));
+  C10_CUDA_CHECK(nvb::launch(sp_join_kernel<HD>, dim3((unsigned)(((long)a.T * a.nq + 3) / 4)), dim3(128), 0, stream, a, pl));
+}
+
+// Tiles per split so that ``groups`` independent row groups over ``tiles`` key tiles make about ``ctas`` CTAs, with at
+// most 32 splits.
+void split_keys(long groups, int tiles, long ctas, int* n, int* per) {
+  *per = (int)std::max<long>(1, std::min<long>(16, groups * tiles / std::max<long>(1, ctas)));
+  *per = std::max(*per, (tiles + 31) / 32);
+  *n = (tiles + *per - 1) / *per;
+}
+
 void check_i32(const at::Tensor& t, const at::Tensor& like, int64_t dim, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.device() == like.device() &&
                   (t.size(-1) <= 1 || t.stride(-1) == 1),
@@ -225,10 +688,29 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
   a.scale = (float)scale, a.softcap = (float)softcap, a.window = (int)window;
   a.err = err.data_ptr<int>();
   auto stream = at::cuda::getCurrentCUDAStream();
-  const long warps = (long)T * nq;
-  C10_CUDA_CHECK(nvb::launch(sp_generic_kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, a,
-                             reinterpret_cast<const bf16*>(k_cache.data_ptr()),
-                             reinterpret_cast<const bf16*>(v_cache.data_ptr())));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {out, 1};
+  if (hd != 64 && hd != 128 && hd != 256) {
+    const long warps = (long)T * nq;
+    C10_CUDA_CHECK(nvb::launch(sp_generic_kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, a,
+                               reinterpret_cast<const bf16*>(k_cache.data_ptr()),
+                               reinterpret_cast<const bf16*>(v_cache.data_ptr())));
+    return {out, 1};
+  }
+  const int G = (int)(nq / nkv), sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int64_t pre_bound = prefix_len_dev.has_value() ? prefix_blocks.numel() * bs : prefix_len;
+  const int pre_tiles = (int)((std::min<int64_t>(pre_bound, max_len) + KT - 1) / KT);
+  const int own_tiles = (int)std::max<int64_t>(0, (max_len + KT - 1) / KT - (prefix_len_dev.has_value() ? 0 : prefix_len / KT));
+  SpPlan pl{};
+  pl.pre_row_tiles = (int)((T * G + kRows - 1) / kRows);
+  pl.own_row_tiles = (int)((std::min(max_q, T) * G + kRows - 1) / kRows);
+  split_keys((long)nkv * pl.pre_row_tiles, pre_tiles, 2 * sms, &pl.n_pre, &pl.pre_tiles);
+  split_keys((long)nkv * B * pl.own_row_tiles, own_tiles, 4 * sms, &pl.n_own, &pl.own_tiles);
+  const int64_t parts = T * nq * (pl.n_pre + pl.n_own);
+  auto scratch = at::empty({parts * (hd + 1)}, q.options().dtype(at::kFloat));
+  pl.part_o = scratch.data_ptr<float>();
+  pl.part_lse = pl.part_o + parts * hd;
+  const void *kp = k_cache.data_ptr(), *vp = v_cache.data_ptr();
+  if (hd == 64) launch_split<64, 4>(a, pl, kp, vp, stream);
+  else if (hd == 128) launch_split<128, 3>(a, pl, kp, vp, stream);
+  else launch_split<256, 2>(a, pl, kp, vp, stream);
+  return {out, 2};
 }
