@@ -147,8 +147,12 @@ constexpr int kCuSmem = 1024;  // sequences whose cu_q fits the shared copy
 struct SpPlan {
   int n_pre, pre_tiles, pre_row_tiles;  // prefix: key splits, tiles per split, row tiles
   int n_own, own_tiles, own_row_tiles;  // own keys: the same, per sequence
-  float* part_o;                        // [T, nq, n_pre + n_own, hd]
-  float* part_lse;                      // [T, nq, n_pre + n_own]
+  int pre_slots;                        // parts of the prefix
+  int tc;                               // the prefix is left to the tcgen05 kernel
+  float* part_o;                        // [T, nq, pre_slots + n_own, hd]
+  float* part_lse;                      // [T, nq, pre_slots + n_own]
+
+  NV_DEVICE int slots() const { return pre_slots + n_own; }
 };
 
 NV_DEVICE int sp_page(const SpArgs& a, const int* pages, int key) {
@@ -366,7 +370,7 @@ __device__ void sp_part_mma(const SpArgs& a, const SpPlan& pl, const SpPart& p, 
     l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
     l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
   }
-  const int NS = pl.n_pre + pl.n_own;
+  const int NS = pl.slots();
   auto slot_of = [&](int r) {
     const int f = p.row0 + r;
     return ((long)(p.tok0 + f / G) * a.nq + p.kvh * G + f % G) * NS + p.slot;
@@ -437,10 +441,8 @@ constexpr size_t sp_mma_smem() {
 // (split, KV head, row tile, sequence).  K/V tiles of 64 keys come through TMA into a ring of STAGES; bound by the
 // bytes of the cache as long as a tile serves few rows.
 template <int HD, int STAGES>
-__global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUtensorMap kmap,
-                                                     const __grid_constant__ CUtensorMap vmap, SpArgs a, SpPlan pl) {
-  nvb::pdl_wait();
-  nvb::pdl_trigger();
+__device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUtensorMap& vmap, const SpArgs& a,
+                                            const SpPlan& pl) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   bf16* qs = reinterpret_cast<bf16*>(ring + STAGES * 2 * KT * HD * 2);
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUt
   const bool p_ok = a.prefix_ok(P);
   SpPart p{};
   int bid = blockIdx.x;
-  const int n_prefix = pl.n_pre * a.nkv * pl.pre_row_tiles;
+  const int n_prefix = pl.tc ? 0 : pl.n_pre * a.nkv * pl.pre_row_tiles;
   const bool is_prefix = bid < n_prefix;
   if (tid == 0) {
     abort_flag = 0;
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUt
     p.row0 = (bid % pl.own_row_tiles) * kRows;
     p.rows = min(kRows, n * G - p.row0);
     if (p.rows <= 0) return;
-    p.slot = pl.n_pre + split;
+    p.slot = pl.pre_slots + split;
     p.klo = P;
     p.kend = ctx;
     p.t0 = P / KT + split * pl.own_tiles;
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUt
   p.t1 = p.kend > p.klo ? min(p.t1, (p.kend + KT - 1) / KT) : p.t0;
   if (a.window > 0 && pos_lo != 0x7fffffff) p.t0 = max(p.t0, max(0, pos_lo - a.window + 1) / KT);
   if (p.t0 >= p.t1) {
-    const int NS = pl.n_pre + pl.n_own;
+    const int NS = pl.slots();
     if (tid < p.rows) {
       const int f = p.row0 + tid;
       pl.part_lse[((long)(p.tok0 + f / G) * a.nq + p.kvh * G + f % G) * NS + p.slot] = -INFINITY;
@@ -531,6 +533,19 @@ __global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUt
   if (p.rows <= 16) sp_part_mma<HD, STAGES, 1>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
   else if (p.rows <= 32) sp_part_mma<HD, STAGES, 2>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
   else sp_part_mma<HD, STAGES, 4>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
+}
+
+template <int HD, int STAGES>
+__global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                     const __grid_constant__ CUtensorMap vmap, const SpArgs a,
+                                                     const SpPlan pl) {
+  // After the tcgen05 kernel nothing here depends on its results: the parts run beside it, on the SMs that it leaves
+  // free.  That kernel has waited for its own predecessor before it let this one start.  The last CTA waits for it at
+  // the end, so that the join, which waits for this kernel, comes after both.
+  if (!pl.tc) nvb::pdl_wait();
+  nvb::pdl_trigger();
+  sp_mma_part<HD, STAGES>(kmap, vmap, a, pl);
+  if (pl.tc && blockIdx.x == gridDim.x - 1) nvb::pdl_wait();
 }
 
 // One warp per (token, head): joins the parts.
@@ -543,7 +558,7 @@ __global__ void __launch_bounds__(128) sp_join_kernel(SpArgs a, SpPlan pl) {
   if (row >= (long)a.T * a.nq) return;
   const int t = (int)(row / a.nq), h = (int)(row % a.nq);
   if (a.cu_q != nullptr && (t < a.cu_q[0] || t >= a.cu_q[a.B])) return;  // a row behind the last sequence
-  const int NS = pl.n_pre + pl.n_own;
+  const int NS = pl.slots();
   const float* lse = pl.part_lse + row * NS;
   const float* po = pl.part_o + row * NS * HD;
   float M = -INFINITY;
@@ -557,19 +572,34 @@ __global__ void __launch_bounds__(128) sp_join_kernel(SpArgs a, SpPlan pl) {
   if (M != -INFINITY)
     for (int s0 = 0; s0 < NS; s0 += 32) {
       const float w = s0 + lane < NS ? exp2f(lse[s0 + lane] - M) : 0.f;
-      for (unsigned left = __ballot_sync(0xffffffffu, w > 0.f); left != 0; left &= left - 1) {
-        const int s = __ffs(left) - 1;
-        const float ws = __shfl_sync(0xffffffffu, w, s);
-        den += ws;
-        const float* src = po + (long)(s0 + s) * HD + lane * PER;
+      den += w;
+      unsigned left = __ballot_sync(0xffffffffu, w > 0.f);
+      while (left != 0) {  // four parts at a time: their loads do not wait for one another
+        int at[4];
+        float ws[4];
 #pragma unroll
-        for (int i = 0; i < PER; i += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(src + i);
-          acc[i] += ws * v.x;
-          acc[i + 1] += ws * v.y;
+        for (int k = 0; k < 4; ++k) {
+          at[k] = left != 0 ? __ffs(left) - 1 : (k > 0 ? at[0] : 0);
+          ws[k] = __shfl_sync(0xffffffffu, w, at[k]);
+          if (left == 0) ws[k] = 0.f;
+          left &= left - 1;
         }
+        float2 v[4][PER / 2];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < PER / 2; ++i)
+            v[k][i] = *reinterpret_cast<const float2*>(po + (long)(s0 + at[k]) * HD + lane * PER + 2 * i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < PER / 2; ++i) {
+            acc[2 * i] += ws[k] * v[k][i].x;
+            acc[2 * i + 1] += ws[k] * v[k][i].y;
+          }
       }
     }
+  den = nvb::warp_sum(den);
   const float inv = den > 0.f ? 1.f / den : 0.f;
   bf16* dst = a.out + t * a.o_tok + h * a.o_head + lane * PER;
 #pragma unroll
@@ -577,17 +607,29 @@ __global__ void __launch_bounds__(128) sp_join_kernel(SpArgs a, SpPlan pl) {
     *reinterpret_cast<uint32_t*>(dst + i) = nvb::pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
 }
 
+#include "shared_prefix_tc.cuh"
+
 template <int HD, int STAGES>
-void launch_split(const SpArgs& a, const SpPlan& pl, const void* kc, const void* vc, cudaStream_t stream) {
+int launch_split(const SpArgs& a, const SpPlan& pl, const void* kc, const void* vc, cudaStream_t stream) {
+  int launches = 1;
   const uint64_t rows = (uint64_t)a.num_blocks * a.nkv * a.block_size;
   const CUtensorMap km = nvb::make_tmap_2d_bf16(kc, rows, HD, HD, KT);
   const CUtensorMap vm = nvb::make_tmap_2d_bf16(vc, rows, HD, HD, KT);
   auto kern = sp_mma_kernel<HD, STAGES>;
   constexpr size_t sm = sp_mma_smem<HD, STAGES>();
   C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
-  const unsigned grid = (unsigned)(pl.n_pre * a.nkv * pl.pre_row_tiles + pl.n_own * a.nkv * pl.own_row_tiles * a.B);
+  if constexpr (HD <= 128) {
+    if (pl.tc) {
+      launch_tc<HD>(a, pl, kc, vc, stream);
+      ++launches;
+    }
+  }
+  const unsigned grid = (unsigned)((pl.tc ? 0 : pl.n_pre * a.nkv * pl.pre_row_tiles) +
+                                   pl.n_own * a.nkv * pl.own_row_tiles * a.B);
+  if (grid > 0) ++launches;
   if (grid > 0) C10_CUDA_CHECK(nvb::launch(kern, dim3(grid), dim3(128), sm, stream, km, vm, a, pl));
   C10_CUDA_CHECK(nvb::launch(sp_join_kernel<HD>, dim3((unsigned)(((long)a.T * a.nq + 3) / 4)), dim3(128), 0, stream, a, pl));
+  return launches;
 }
 
 // Tiles per split so that ``groups`` independent row groups over ``tiles`` key tiles make about ``ctas`` CTAs, with at
@@ -697,20 +739,32 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
   }
   const int G = (int)(nq / nkv), sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   const int64_t pre_bound = prefix_len_dev.has_value() ? prefix_blocks.numel() * bs : prefix_len;
-  const int pre_tiles = (int)((std::min<int64_t>(pre_bound, max_len) + KT - 1) / KT);
+  const int64_t pre_keys = std::min<int64_t>(pre_bound, max_len);
   const int own_tiles = (int)std::max<int64_t>(0, (max_len + KT - 1) / KT - (prefix_len_dev.has_value() ? 0 : prefix_len / KT));
   SpPlan pl{};
-  pl.pre_row_tiles = (int)((T * G + kRows - 1) / kRows);
+  const int64_t rows = T * G;
+  pl.tc = pre_keys > 0 && hd <= 128 && bs % 128 == 0 && rows > 64;
+  if (pl.tc) {
+    pl.pre_row_tiles = (int)((rows + 255) / 256);
+    const int tiles = (int)((pre_keys + 127) / 128);
+    int n = std::max<int>(1, sms / (int)(nkv * pl.pre_row_tiles));
+    pl.pre_tiles = (tiles + n - 1) / n;
+    pl.n_pre = (tiles + pl.pre_tiles - 1) / pl.pre_tiles;
+    pl.pre_slots = 2 * pl.n_pre;
+  } else {
+    pl.pre_row_tiles = (int)((rows + kRows - 1) / kRows);
+    split_keys((long)nkv * pl.pre_row_tiles, (int)((pre_keys + KT - 1) / KT), 2 * sms, &pl.n_pre, &pl.pre_tiles);
+    pl.pre_slots = pl.n_pre;
+  }
   pl.own_row_tiles = (int)((std::min(max_q, T) * G + kRows - 1) / kRows);
-  split_keys((long)nkv * pl.pre_row_tiles, pre_tiles, 2 * sms, &pl.n_pre, &pl.pre_tiles);
   split_keys((long)nkv * B * pl.own_row_tiles, own_tiles, 4 * sms, &pl.n_own, &pl.own_tiles);
-  const int64_t parts = T * nq * (pl.n_pre + pl.n_own);
+  const int64_t parts = T * nq * (pl.pre_slots + pl.n_own);
   auto scratch = at::empty({parts * (hd + 1)}, q.options().dtype(at::kFloat));
   pl.part_o = scratch.data_ptr<float>();
   pl.part_lse = pl.part_o + parts * hd;
   const void *kp = k_cache.data_ptr(), *vp = v_cache.data_ptr();
-  if (hd == 64) launch_split<64, 4>(a, pl, kp, vp, stream);
-  else if (hd == 128) launch_split<128, 3>(a, pl, kp, vp, stream);
-  else launch_split<256, 2>(a, pl, kp, vp, stream);
-  return {out, 2};
+  const int launches = hd == 64    ? launch_split<64, 4>(a, pl, kp, vp, stream)
+                       : hd == 128 ? launch_split<128, 3>(a, pl, kp, vp, stream)
+                                   : launch_split<256, 2>(a, pl, kp, vp, stream);
+  return {out, launches};
 }

@@ -1,0 +1,546 @@
+// The prefix's part of shared-prefix attention on the 5th-generation tensor cores.  Included by shared_prefix.cu.
+//
+// All query rows (token, head of the GQA group) of the batch stand against the same keys, so they fill MMA tiles of 128
+// rows whatever sequence they come from.  One CTA per (range of keys, KV head, 256 rows) works on two tiles at once:
+// while the softmax threads of one turn its scores into weights, the tensor cores run the other's products.
+//   S_q = Q_q K^T    operands in shared memory, fp32 scores in tensor memory (128 columns per tile)
+//   P_q = 2^(S - m)  one thread per row: scores from tensor memory twice (maximum, then weights), P back as bf16 over the
+//                    first half of the scores' columns
+//   O_q += P_q V     A = P from tensor memory, B = V in shared memory, fp32 O in tensor memory
+// With more than 128 rows the two tiles are rows [0, 128) and [128, 256) against every key tile; with fewer, both are
+// the same rows, one against the even key tiles of the range, the other against the odd ones, and each writes a part.
+// The maximum in use moves (and O, l are rescaled) only when a row's maximum grows by more than 2^8: weights stay
+// below 2^8 and O / l is exact all the same.  Both products of a tile take as long as its exponentials (head dim 128:
+// 1024 clocks each), so the kernel is bound by either pipe at best.
+//
+// Warps: 0 / 3 copy K / V tiles (TMA), 1 issues the MMAs, 2 does the issuer's waits (an mbarrier wait in the issuing
+// thread after a batch of MMAs returns only when the batch has drained) and clears the V rows behind the prefix, 4-7 and
+// 8-11 are the softmax threads of the two tiles.  Every wait is bounded.
+#pragma once
+
+template <int HD>
+struct SpTc {
+  static constexpr int BN = 128;
+  static constexpr int KS = HD == 64 ? 4 : 3, VS = HD == 64 ? 4 : 2;
+  static constexpr int KBOX = BN * 128;           // 64 dims of a K or V tile, bytes
+  static constexpr int KTILE = (HD / 64) * KBOX;
+  static constexpr int QBOX = 128 * 128;          // 64 dims of 128 query rows
+  static constexpr int QTILE = (HD / 64) * QBOX;
+  static constexpr uint32_t O_COL = 2 * BN;       // tensor memory: S of both tiles, then O of both
+  static_assert(O_COL + 2 * HD <= 512, "tensor memory plan");
+  static constexpr int kBars = 2 * KS + 2 * VS + 14;
+  static constexpr size_t smem() { return 1024 + 2 * QTILE + (size_t)(KS + VS) * KTILE + kBars * 8; }
+};
+
+NV_DEVICE void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+NV_DEVICE void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+NV_DEVICE void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+NV_DEVICE void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D(tmem) (+)= A(tmem) B(smem), bf16 operands
+NV_DEVICE void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// V as an MN-major operand: rows (keys) along K in 8-row swizzle atoms, 64-dim boxes ``mn_stride`` bytes apart along N.
+NV_DEVICE uint64_t tc_desc_v(uint32_t addr, uint32_t mn_stride) {
+  uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((mn_stride >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+// Barrier of the issuing and the waiting warp; true when neither has failed.
+NV_DEVICE bool tc_handoff(int ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred pi, po;\n\tsetp.ne.u32 pi, %1, 0;\n\t"
+      "bar.red.and.pred po, 2, 64, pi;\n\tselp.u32 %0, 1, 0, po;\n\t}"
+      : "=r"(r)
+      : "r"(ok)
+      : "memory");
+  return r != 0;
+}
+
+// two fp32 values in one register pair, and operations on both at once
+NV_DEVICE uint64_t pack2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+NV_DEVICE void unpack2(uint64_t d, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d)); }
+NV_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+NV_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Sequence of the warp's first token by a 32-way search, then each lane walks on to its own token (consecutive tokens
+// of a warp lie in the same or the next sequences).
+NV_DEVICE int warp_row_position(const SpArgs& a, int t_first, int t, int P) {
+  if (a.cu_q == nullptr) return row_position(a, nullptr, t, P);
+  const int lane = threadIdx.x & 31;
+  int lo = 0, len = a.B;
+  while (len > 1) {  // cu_q[lo] <= t_first; the answer lies in [lo, lo + len)
+    const int step = (len + 31) / 32, at = lo + lane * step;
+    const bool below = at < lo + len && a.cu_q[at] <= t_first;
+    const int n = __popc(__ballot_sync(0xffffffffu, below));
+    const int skip = max(0, n - 1) * step;
+    lo += skip;
+    len = min(step, len - skip);
+  }
+  if (t >= a.T) return -1;
+  int b = lo;
+  while (b + 1 < a.B && a.cu_q[b + 1] <= t) ++b;
+  const int c0 = a.cu_q[b], c1 = a.cu_q[b + 1];
+  if (c0 < 0 || c1 > a.T || t < c0 || t >= c1 || c1 - c0 > a.max_q) return -1;
+  const int ctx = a.ctx_lens[b];
+  return a.ctx_ok(ctx, P) ? ctx - (c1 - c0) + (t - c0) : -1;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                       const __grid_constant__ CUtensorMap vmap, const SpArgs a,
+                                                       const SpPlan pl) {
+  using C = SpTc<HD>;
+  constexpr int BN = C::BN, KS = C::KS, VS = C::VS;
+  constexpr uint32_t IDESC_S = nvb::idesc_bf16_f32(128, BN);
+  constexpr uint32_t IDESC_PV = nvb::idesc_bf16_f32(128, HD) | (1u << 16);  // V is MN-major
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* kring = qs + 2 * C::QTILE;
+  uint8_t* vring = kring + (size_t)KS * C::KTILE;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(vring + (size_t)VS * C::KTILE);
+  uint64_t* k_free = k_full + KS;
+  uint64_t* v_full = k_free + KS;
+  uint64_t* v_free = v_full + VS;
+  uint64_t* s_full = v_free + VS;  // [2] scores of a tile
+  uint64_t* p_full = s_full + 2;   // [2] its weights
+  uint64_t* o_done = p_full + 2;   // [2] its product with V
+  uint64_t* turn = o_done + 2;     // [2][4] a warp's turn at the exponentials
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ int abort_flag, pos_lo, pos_hi;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    abort_flag = 0;
+    pos_lo = 0x7fffffff;
+    pos_hi = -1;
+    for (int s = 0; s < KS; ++s) {
+      nvb::mbar_init(&k_full[s], 1);
+      nvb::mbar_init(&k_free[s], 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      nvb::mbar_init(&v_full[s], 1);
+      nvb::mbar_init(&v_free[s], 1);
+    }
+    for (int q = 0; q < 2; ++q) {
+      nvb::mbar_init(&s_full[q], 1);
+      nvb::mbar_init(&p_full[q], 4);
+      nvb::mbar_init(&o_done[q], 1);
+      for (int w = 0; w < 4; ++w) nvb::mbar_init(&turn[q * 4 + w], 1);
+    }
+    nvb::fence_mbar_init();
+    nvb::tma_prefetch_desc(&kmap);
+    nvb::tma_prefetch_desc(&vmap);
+  }
+  if (warp == 1) {
+    nvb::tmem_alloc(&tmem_base_sh, 512);
+    nvb::tmem_relinquish();
+  }
+  nvb::pdl_wait();
+  nvb::pdl_trigger();
+
+  const int G = a.nq / a.nkv, P = a.prefix_len();
+  int bid = blockIdx.x;
+  const int split = bid % pl.n_pre;
+  bid /= pl.n_pre;
+  const int kvh = bid % a.nkv, row0 = (bid / a.nkv) * 256;
+  const int rows = min(256, a.T * G - row0);
+  const bool twice = rows <= 128;  // both tiles are the same rows
+  const int kend = a.prefix_ok(P) ? P : 0;
+  int t0 = split * pl.pre_tiles;
+  const int t1 = min(t0 + pl.pre_tiles, (kend + BN - 1) / BN);
+  // one K or V tile into its ring
+  auto copy = [&](bool is_k, int i) {
+    const int s = i % (is_k ? KS : VS), tok = (t0 + i) * BN;
+    const int row = (sp_page(a, a.prefix_blocks, tok) * a.nkv + kvh) * a.block_size + tok % a.block_size;
+    uint8_t* dst = (is_k ? kring : vring) + (size_t)s * C::KTILE;
+    uint64_t* bar = is_k ? &k_full[s] : &v_full[s];
+    nvb::mbar_arrive_expect_tx(bar, C::KTILE);
+#pragma unroll
+    for (int j = 0; j < HD / 64; ++j) nvb::tma_load_2d(dst + j * C::KBOX, is_k ? &kmap : &vmap, bar, j * 64, row);
+  };
+  const bool early = a.window <= 0;  // the first key tile is known before the rows' positions are
+  if (tid == 0) {
+    if (!a.prefix_ok(P)) nvb::record_error(a.err, nvb::kErrBadArgument);
+    if (early) {
+      for (int i = 0; i < KS && i < t1 - t0; ++i) copy(true, i);
+      for (int i = 0; i < VS && i < t1 - t0; ++i) copy(false, i);
+    }
+  }
+  // The softmax threads load the query rows, into the swizzled layout that the MMA reads (zeros behind the list), and
+  // find the rows' positions.
+  const int tile = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;  // warps 4-11
+  const int rr = row0 + (twice ? 0 : tile * 128) + r;             // row of the list
+  int pos = -1;                                                   // no key seen
+  if (warp >= 4) {
+    if (!(twice && tile == 1)) {
+      constexpr int CH = HD / 8, STEP = 128 / CH;  // 16-byte chunks of a row; rows that the 128 threads load at once
+      const int c = tid % CH, first = (tid & 127) / CH;
+      uint8_t* qt = qs + tile * C::QTILE + (c >> 3) * C::QBOX;
+      const bf16* src = a.q + (long)kvh * G * a.q_head + c * 8;
+      uint4 v[CH];
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const int f = row0 + tile * 128 + first + k * STEP;
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (f < row0 + rows) v[k] = *reinterpret_cast<const uint4*>(src + (long)(f / G) * a.q_tok + (long)(f % G) * a.q_head);
+      }
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+        *reinterpret_cast<uint4*>(qt + nvb::swz128(first + k * STEP, c & 7)) = v[k];
+      nvb::fence_proxy_async();
+    }
+    const int first = row0 + (twice ? 0 : tile * 128) + (warp & 3) * 32;
+    if (first < row0 + rows) {
+      pos = warp_row_position(a, first / G, rr / G, P);
+      if (rr >= row0 + rows) pos = -1;
+    }
+    if (!early) {
+      const int lo = __reduce_min_sync(0xffffffffu, pos < 0 ? 0x7fffffff : pos);
+      const int hi = __reduce_max_sync(0xffffffffu, pos);
+      if (lane == 0 && hi >= 0) {
+        atomicMin(&pos_lo, lo);
+        atomicMax(&pos_hi, hi);
+      }
+    }
+  }
+  nvb::tc_fence_before();
+  __syncthreads();
+  nvb::tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+  // with a window: only the key tiles that some row sees
+  if (!early) t0 = pos_hi < 0 ? t1 : max(t0, max(0, pos_lo - a.window + 1) / BN);
+  const int nt = max(0, t1 - t0);
+  // step j of tile q works on key tile t0 + j, or t0 + 2 j + q
+  const int stride = twice ? 2 : 1;
+  const int steps0 = twice ? (nt + 1) / 2 : nt, steps1 = twice ? nt / 2 : nt;
+
+  // registers: launched with 168 a thread (64512 in all); 128 * 88 + 256 * 208 is the same sum
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp == 0 || warp == 3) {
+    // ---------------------------------------------------------------- copies
+    const bool is_k = warp == 0;
+    if (lane == 0) {
+      const int NS = is_k ? KS : VS;
+      uint64_t* full = is_k ? k_full : v_full;
+      uint64_t* freeb = is_k ? k_free : v_free;
+      int i = early ? min(NS, nt) : 0;
+      bool ok = true;
+      for (; i < nt; ++i) {
+        if (i >= NS && !nvb::mbar_wait(&freeb[i % NS], ((i / NS) & 1) ^ 1, a.err, &abort_flag)) {
+          ok = false;
+          break;
+        }
+        copy(is_k, i);
+      }
+      if (!ok)  // bounded drain of copies that may still be landing
+        for (int j = (i > NS ? i - NS : 0); j < i; ++j) nvb::mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, nullptr);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issue
+    // key tile i against Q tile q
+    auto issue_s = [&](int q, int i, bool last_use) {
+      const uint32_t ka = nvb::smem_u32(kring + (size_t)(i % KS) * C::KTILE);
+      const uint32_t qa = nvb::smem_u32(qs) + (twice ? 0 : q) * C::QTILE;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk)
+        nvb::tc_mma_f16(tmem + (uint32_t)q * BN, nvb::sdesc_kmajor_sw128(qa + (kk >> 2) * C::QBOX + (kk & 3) * 32),
+                        nvb::sdesc_kmajor_sw128(ka + (kk >> 2) * C::KBOX + (kk & 3) * 32), IDESC_S, kk > 0 ? 1u : 0u);
+      nvb::tc_commit(&s_full[q]);
+      if (last_use) nvb::tc_commit(&k_free[i % KS]);
+    };
+    auto issue_pv = [&](int q, int i, bool first, bool last_use) {
+      const uint32_t va = nvb::smem_u32(vring + (size_t)(i % VS) * C::KTILE);
+#pragma unroll
+      for (int kk = 0; kk < BN / 16; ++kk)
+        tc_mma_ts(tmem + C::O_COL + (uint32_t)q * HD, tmem + (uint32_t)q * BN + kk * 8,
+                  tc_desc_v(va + kk * 2048, C::KBOX), IDESC_PV, (!first || kk > 0) ? 1u : 0u);
+      nvb::tc_commit(&o_done[q]);
+      if (last_use) nvb::tc_commit(&v_free[i % VS]);
+    };
+    bool ok = nt > 0;
+    for (int q = 0; ok && q < 2; ++q) {  // scores of both tiles' first steps
+      if (q == 1 && steps1 == 0) break;
+      ok = tc_handoff(1);
+      if (!ok) break;
+      nvb::tc_fence_after();
+      if (lane == 0) issue_s(q, twice ? q : 0, twice || q == 1);
+      __syncwarp();
+    }
+    for (int j = 0; ok && j < steps0; ++j)
+      for (int q = 0; ok && q < 2; ++q) {
+        if (q == 1 && j >= steps1) break;
+        ok = tc_handoff(1);  // P of this step is in tensor memory, V landed; the next K tile landed
+        if (!ok) break;
+        nvb::tc_fence_after();
+        if (lane == 0) {
+          const int i = j * stride + (twice ? q : 0);
+          issue_pv(q, i, j == 0, twice || q == 1);
+          // the next scores overwrite P: the tensor pipe runs MMAs in the order of issue
+          if (j + 1 < (q == 0 ? steps0 : steps1)) issue_s(q, i + stride, twice || q == 1);
+        }
+        __syncwarp();
+      }
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- the issuer's waits
+    bool ok = nt > 0;
+    auto wait = [&](uint64_t* bar, int phase) {
+      int o = 1;
+      if (lane == 0) o = nvb::mbar_wait(bar, (uint32_t)(phase & 1), a.err, &abort_flag) ? 1 : 0;
+      return __shfl_sync(0xffffffffu, o, 0) != 0;
+    };
+    for (int q = 0; ok && q < 2; ++q) {
+      if (q == 1 && steps1 == 0) break;
+      const int i = twice ? q : 0;
+      ok = tc_handoff(wait(&k_full[i % KS], i / KS));
+    }
+    for (int j = 0; ok && j < steps0; ++j)
+      for (int q = 0; ok && q < 2; ++q) {
+        if (q == 1 && j >= steps1) break;
+        const int i = j * stride + (twice ? q : 0);
+        bool good = wait(&v_full[i % VS], i / VS);
+        const int tok0 = (t0 + i) * BN;
+        if (good && tok0 + BN > kend && (twice || q == 0)) {
+          // keys behind the prefix may hold anything: their weight is 0, and 0 * NaN must not reach the sum
+          uint8_t* vt = vring + (size_t)(i % VS) * C::KTILE;
+          for (int x = lane + (kend - tok0) * (HD / 8); x < BN * (HD / 8); x += 32) {
+            const int vr = x / (HD / 8), c = x % (HD / 8);
+            *reinterpret_cast<uint4*>(vt + (c >> 3) * C::KBOX + nvb::swz128(vr, c & 7)) = make_uint4(0, 0, 0, 0);
+          }
+          nvb::fence_proxy_async();
+        }
+        good = good && wait(&p_full[q], j);
+        if (j + 1 < (q == 0 ? steps0 : steps1)) good = good && wait(&k_full[(i + stride) % KS], (i + stride) / KS);
+        ok = tc_handoff(good);
+      }
+  }
+  } else {
+    // ---------------------------------------------------------------- softmax and output
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int steps = tile == 0 ? steps0 : steps1;
+    const bool have = rr < row0 + rows;
+    const int t = rr / G, h = kvh * G + rr % G;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_col = lanes + (uint32_t)tile * BN, o_col = lanes + C::O_COL + (uint32_t)tile * HD;
+    const float sl2 = a.scale * kLog2e;
+    const int win = a.window > 0 ? a.window : 0x40000000;
+    const bool linear = a.softcap <= 0.f && sl2 > 0.f;  // then the maximum may be taken before the scale
+    const float mul = linear ? sl2 : 1.f;
+    const bool idle = !have || t >= a.T;  // nothing is written for the row: no need to mask it
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    // The warps of the two tiles that share an SM quarter take turns at the exponentials: left alone they run in step,
+    // and the tensor cores wait for both and then both for the tensor cores.
+    uint64_t* my_turn = &turn[tile * 4 + (warp & 3)];
+    uint64_t* other_turn = &turn[(tile ^ 1) * 4 + (warp & 3)];
+    for (int j = 0; j < steps; ++j) {
+      int okw = 1;
+      if (lane == 0) {
+        okw = nvb::mbar_wait(&s_full[tile], (uint32_t)(j & 1), a.err, &abort_flag) ? 1 : 0;
+        if (tile == 1) okw = okw && nvb::mbar_wait(my_turn, (uint32_t)(j & 1), a.err, &abort_flag);
+        else if (j > 0 && j <= steps1) okw = okw && nvb::mbar_wait(my_turn, (uint32_t)((j - 1) & 1), a.err, &abort_flag);
+      }
+      if (!__shfl_sync(0xffffffffu, okw, 0)) {
+        ok = false;
+        break;
+      }
+      nvb::tc_fence_after();
+      uint32_t u[BN];
+#pragma unroll
+      for (int c = 0; c < BN; c += 32) tc_ld32(s_col + c, *reinterpret_cast<uint32_t(*)[32]>(u + c));
+      nvb::tmem_ld_wait();
+      nvb::reg_fence<BN>(u);
+      const int key0 = (t0 + j * stride + (twice ? tile : 0)) * BN;
+      auto val = [&](int e) { return __uint_as_float(u[e]); };
+      if (!linear) {
+        if (a.softcap > 0.f) {
+#pragma unroll
+          for (int e = 0; e < BN; ++e) u[e] = __float_as_uint(sp_cap(val(e) * a.scale, a.softcap) * kLog2e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < BN; ++e) u[e] = __float_as_uint(val(e) * sl2);
+        }
+      }
+      // columns (lo, hi] are seen; a key tile that every row of this warp sees whole skips the masks
+      const int hi = min(kend - 1, pos) - key0, lo = pos - win - key0;
+      if (!__all_sync(0xffffffffu, idle || (hi >= BN - 1 && lo < 0))) {
+#pragma unroll
+        for (int e = 0; e < BN; ++e) u[e] = e <= hi && e > lo ? u[e] : 0xff800000u;
+      }
+      float m4[4] = {val(0), val(1), val(2), val(3)};
+#pragma unroll
+      for (int e = 4; e < BN; ++e) m4[e & 3] = fmaxf(m4[e & 3], val(e));
+      const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+      float new_m = m_used;
+      bool need = false;
+      if (mt > -INFINITY) {
+        if (m_used == -INFINITY) {
+          new_m = mt;  // the O row is still zero
+        } else if (mt > m_used + 8.f) {
+          new_m = mt;
+          need = true;
+        }
+      }
+      if (__any_sync(0xffffffffu, need)) {  // j >= 1 here
+        okw = 1;
+        if (lane == 0) okw = nvb::mbar_wait(&o_done[tile], (uint32_t)((j - 1) & 1), a.err, &abort_flag) ? 1 : 0;
+        if (!__shfl_sync(0xffffffffu, okw, 0)) {
+          ok = false;
+          break;
+        }
+        nvb::tc_fence_after();
+        const float f = need ? exp2f(m_used - new_m) : 1.f;
+        l *= f;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t u[32];
+          tc_ld32(o_col + c, u);
+          nvb::tmem_ld_wait();
+          nvb::reg_fence<32>(u);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
+          tc_st32(o_col + c, u);
+        }
+        tc_st_wait();
+      }
+      m_used = new_m;
+      const float mneg = m_used == -INFINITY ? 0.f : -m_used;  // a row without keys: every score is -inf, every weight 0
+      const uint64_t mul2 = pack2(mul, mul), neg2 = pack2(mneg, mneg);
+      uint64_t rs0 = 0, rs1 = 0;
+#pragma unroll
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float p[4];
+          unpack2(fma2(pack2(val(c + e), val(c + e + 1)), mul2, neg2), p[0], p[1]);
+          unpack2(fma2(pack2(val(c + e + 2), val(c + e + 3)), mul2, neg2), p[2], p[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = exp2f(p[i]);
+          rs0 = add2(rs0, pack2(p[0], p[1]));
+          rs1 = add2(rs1, pack2(p[2], p[3]));
+          w[e / 2] = nvb::pack_bf16x2(p[0], p[1]);
+          w[e / 2 + 1] = nvb::pack_bf16x2(p[2], p[3]);
+        }
+        tc_st16(s_col + c / 2, w);  // over the scores, which are in registers
+      }
+      __syncwarp();
+      if (lane == 0) nvb::mbar_arrive(other_turn);
+      float r0, r1;
+      unpack2(add2(rs0, rs1), r0, r1);
+      l += r0 + r1;
+      tc_st_wait();
+      nvb::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) nvb::mbar_arrive(&p_full[tile]);
+    }
+    // the part: O / l and the log2-sum-exp
+    int okw = ok ? 1 : 0;
+    if (ok && steps > 0 && lane == 0) okw = nvb::mbar_wait(&o_done[tile], (uint32_t)((steps - 1) & 1), a.err, &abort_flag) ? 1 : 0;
+    okw = __shfl_sync(0xffffffffu, okw, 0);
+    nvb::tc_fence_after();
+    if (okw) {
+      const int NS = pl.slots(), part = 2 * split + (twice ? tile : 0);
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      if (have) {
+        const long slot = ((long)t * a.nq + h) * NS + part;
+        pl.part_lse[slot] = l > 0.f ? m_used + log2f(l) : -INFINITY;
+        if (!twice) pl.part_lse[slot + 1] = -INFINITY;
+      }
+      if (steps > 0) {
+        // 16 columns at a time through shared memory, so that four lanes write 64 consecutive bytes of a row.  The space
+        // is this tile's Q (its products are done), with one set of rows the second Q tile, which is not used.
+        uint8_t* st = qs + (twice ? C::QTILE + (warp - 4) * 2048 : tile * C::QTILE + (warp & 3) * 2048);
+        float* dst[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int f = rr - lane + k * 8 + (lane >> 2);
+          dst[k] = f < row0 + rows
+                       ? pl.part_o + (((long)(f / G) * a.nq + kvh * G + f % G) * NS + part) * HD + (lane & 3) * 4
+                       : nullptr;
+        }
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 16) {
+          uint32_t u[16];
+          nvb::tmem_ld_32x32b_x16(o_col + c, u);
+          nvb::tmem_ld_wait();
+          nvb::reg_fence<16>(u);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float4*>(st + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
+                make_float4(__uint_as_float(u[4 * k]) * inv, __uint_as_float(u[4 * k + 1]) * inv,
+                            __uint_as_float(u[4 * k + 2]) * inv, __uint_as_float(u[4 * k + 3]) * inv);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = k * 8 + (lane >> 2);
+            const float4 v = *reinterpret_cast<const float4*>(st + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+            if (dst[k] != nullptr) *reinterpret_cast<float4*>(dst[k] + c) = v;
+          }
+        }
+      }
+    }
+  }
+  nvb::tc_fence_before();
+  __syncthreads();
+  nvb::tc_fence_after();
+  if (warp == 1) nvb::tmem_dealloc(tmem, 512);
+}
+
+template <int HD>
+void launch_tc(const SpArgs& a, const SpPlan& pl, const void* kc, const void* vc, cudaStream_t stream) {
+  const uint64_t rows = (uint64_t)a.num_blocks * a.nkv * a.block_size;
+  const CUtensorMap km = nvb::make_tmap_2d_bf16(kc, rows, HD, HD, SpTc<HD>::BN);
+  const CUtensorMap vm = nvb::make_tmap_2d_bf16(vc, rows, HD, HD, SpTc<HD>::BN);
+  auto kern = sp_tc_kernel<HD>;
+  constexpr size_t sm = SpTc<HD>::smem();
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+  C10_CUDA_CHECK(nvb::launch(kern, dim3((unsigned)(pl.n_pre * a.nkv * pl.pre_row_tiles)), dim3(384), sm, stream, km, vm, a, pl));
+}

@@ -140,6 +140,33 @@ def test_sequences_shorter_than_the_prefix(nq, nkv, hd, dev):
     assert bool((got[2] == 0).all()) and bool((got[5:7] == 0).all())
 
 
+@gpu
+@pytest.mark.parametrize("rows", [17, 32, 33, 64, 65, 150])
+@pytest.mark.parametrize("prefix", [1, 127, 128, 129, 700, 1536])
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 128), (4, 1, 64), (4, 1, 256)])
+def test_many_rows(rows, prefix, nq, nkv, hd):
+    """Batches that fill one or several tiles of query rows against the prefix; uneven numbers of query tokens."""
+    qs, n = [], 0
+    while n < rows:
+        qs.append(min(rows - n, (0, 1, 3, 2, 1, 5)[len(qs) % 6]))
+        n += qs[-1]
+    owns = [q + (0, 7, 64, 130)[i % 4] for i, q in enumerate(qs)]
+    s = make(prefix, owns, qs, nq, nkv, hd, seed=rows + prefix)
+    check(call(s, "cuda", hd ** -0.5), s, hd ** -0.5)
+
+
+@gpu
+@pytest.mark.parametrize("window,softcap,amp,scale", [(90, 0.0, 1.0, 0.1), (600, 0.0, 1.0, 0.1), (0, 15.0, 3.0, 0.1),
+                                                      (0, 0.0, 3.0, 0.1), (0, 0.0, 1.0, -0.1), (0, 0.0, 1.0, 0.0)])
+@pytest.mark.parametrize("batch", [30, 80])
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 128), (8, 2, 64), (4, 1, 256)])
+def test_many_rows_masks_and_scales(window, softcap, amp, scale, batch, nq, nkv, hd):
+    """Windows that leave rows without a key of the prefix, contexts inside it, soft-caps, moving maxima, any scale."""
+    owns = [(1, 5, 700, 64, -300, -899, -900)[i % 7] for i in range(batch)]
+    s = make(900, owns, [1] * batch, nq, nkv, hd, seed=batch, amp=amp)
+    check(call(s, "cuda", scale, window=window, softcap=softcap), s, scale, softcap, window)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_large_scores(dev):
     """Scores spread over tens of units: the running maximum moves from tile to tile."""
@@ -303,7 +330,7 @@ def test_long_offsets():
 @pytest.mark.parametrize("hd", [64, 128, 256, 512])
 def test_streams_and_graphs(hd):
     """Two calls on two streams at once, and two captured graphs replayed together, give the single call's bits."""
-    cases = [make(1200, [300, 60, 9] * 4, [1, 2, 3] * 4, 8, 2, hd, seed=i) for i in range(2)]
+    cases = [make(1200, [300, 60, 9] * 8, [1, 2, 3] * 8, 8, 2, hd, seed=i) for i in range(2)]
     dev = [{k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in s.items()} for s in cases]
     f = lambda d: ops.shared_prefix_attention(scale=hd ** -0.5, **d)  # noqa: E731
     want = [f(d) for d in dev]
@@ -336,10 +363,11 @@ def test_streams_and_graphs(hd):
 
 
 @gpu
-def test_graph_follows_lengths_on_the_device():
+@pytest.mark.parametrize("many", [3, 30])
+def test_graph_follows_lengths_on_the_device(many):
     """A captured call replayed with another prefix length, contexts and pages."""
-    a = make(900, [30, 200], [1, 2], 8, 2, 128, seed=1, spare=3)
-    b = make(640, [290, 3], [1, 2], 8, 2, 128, seed=2, spare=4)
+    a = make(900, [30, 200], [1, many - 1], 8, 2, 128, seed=1, spare=3)
+    b = make(640, [290, 40], [many - 2, 2], 8, 2, 128, seed=2, spare=4)
     buf = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in a.items()}
     buf["k_cache"] = torch.zeros(12, 2, BS, 128, dtype=torch.bfloat16, device="cuda")
     buf["v_cache"] = torch.zeros_like(buf["k_cache"])
@@ -356,6 +384,7 @@ def test_graph_follows_lengths_on_the_device():
         buf["prefix_len"].fill_(s["prefix_len"])
 
     load(a)
+    buf["max_q"] = many
     f = lambda: ops.shared_prefix_attention(scale=128 ** -0.5, max_len=2048, **buf)  # noqa: E731
     f()
     torch.cuda.synchronize()
