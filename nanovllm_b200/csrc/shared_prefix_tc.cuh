@@ -13,9 +13,8 @@
 // below 2^8 and O / l is exact all the same.  Both products of a tile take as long as its exponentials (head dim 128:
 // 1024 clocks each), so the kernel is bound by either pipe at best.
 //
-// Warps: 0 / 3 copy K / V tiles (TMA), 1 issues the MMAs, 2 does the issuer's waits (an mbarrier wait in the issuing
-// thread after a batch of MMAs returns only when the batch has drained) and clears the V rows behind the prefix, 4-7 and
-// 8-11 are the softmax threads of the two tiles.  Every wait is bounded.
+// Warps: 0 / 3 copy K / V tiles (TMA), 1 issues the MMAs, 2 clears the V rows behind the prefix, 4-7 and 8-11 are the
+// softmax threads of the two tiles.  Every wait is bounded.
 #pragma once
 
 template <int HD>
@@ -28,7 +27,7 @@ struct SpTc {
   static constexpr int QTILE = (HD / 64) * QBOX;
   static constexpr uint32_t O_COL = 2 * BN;       // tensor memory: S of both tiles, then O of both
   static_assert(O_COL + 2 * HD <= 512, "tensor memory plan");
-  static constexpr int kBars = 2 * KS + 2 * VS + 14;
+  static constexpr int kBars = 2 * KS + 2 * VS + 7;
   static constexpr size_t smem() { return 1024 + 2 * QTILE + (size_t)(KS + VS) * KTILE + kBars * 8; }
 };
 
@@ -70,6 +69,13 @@ NV_DEVICE void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc
       "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// True in one lane of a converged warp, always the same one.  The MMAs stand in a branch on it and not on lane == 0:
+// measured beside busy softmax warps, an issue then costs 85-100 cycles against 170 (64 either way on a quiet SM).
+NV_DEVICE bool tc_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // V as an MN-major operand: rows (keys) along K in 8-row swizzle atoms, 64-dim boxes ``mn_stride`` bytes apart along N.
 NV_DEVICE uint64_t tc_desc_v(uint32_t addr, uint32_t mn_stride) {
   uint64_t d = (uint64_t)((addr >> 4) & 0x3FFFu);
@@ -79,16 +85,12 @@ NV_DEVICE uint64_t tc_desc_v(uint32_t addr, uint32_t mn_stride) {
   d |= (uint64_t)2u << 61;
   return d;
 }
-// Barrier of the issuing and the waiting warp; true when neither has failed.
-NV_DEVICE bool tc_handoff(int ok) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred pi, po;\n\tsetp.ne.u32 pi, %1, 0;\n\t"
-      "bar.red.and.pred po, 2, 64, pi;\n\tselp.u32 %0, 1, 0, po;\n\t}"
-      : "=r"(r)
-      : "r"(ok)
-      : "memory");
-  return r != 0;
+// Bounded wait that looks at the barrier a few times before it reads the clock (which takes longer than most waits).
+NV_DEVICE bool tc_wait(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i)
+    if (nvb::mbar_try_wait(bar, parity)) return true;
+  return nvb::mbar_wait(bar, parity, err, abort_flag);
 }
 
 // two fp32 values in one register pair, and operations on both at once
@@ -107,6 +109,28 @@ NV_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+
+// 2^v of two values on the FMA pipe, for a part of the weights: the special-function unit gives 16 a clock and SM, which
+// for a whole tile is as long as the tile's products.  v = n + f with n the nearest integer (from the low bits of
+// v + 1.5 * 2^23), 2^f by a polynomial of degree 4 fitted to the relative error on [-1/2, 1/2] (2.7e-6, far below the
+// bf16 that the weight is rounded to), n added to the exponent.  Below -126 the result is 2^-126 instead of less.
+NV_DEVICE void exp2_poly2(uint64_t v, float& p0, float& p1) {
+  float x0, x1;
+  unpack2(v, x0, x1);
+  v = pack2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t magic = pack2(12582912.f, 12582912.f), back = pack2(-12582912.f, -12582912.f);
+  const uint64_t n = add2(v, magic);
+  const uint64_t f = fma2(add2(n, back), pack2(-1.f, -1.f), v);
+  uint64_t y = fma2(f, pack2(0.00957010221f, 0.00957010221f), pack2(0.0559178628f, 0.0559178628f));
+  y = fma2(f, y, pack2(0.240247443f, 0.240247443f));
+  y = fma2(f, y, pack2(0.693121791f, 0.693121791f));
+  y = fma2(f, y, pack2(0.999999285f, 0.999999285f));
+  float n0, n1, y0, y1;
+  unpack2(n, n0, n1);
+  unpack2(y, y0, y1);
+  p0 = __int_as_float((__float_as_int(n0) << 23) + __float_as_int(y0));
+  p1 = __int_as_float((__float_as_int(n1) << 23) + __float_as_int(y1));
 }
 
 // Sequence of the warp's first token by a 32-way search, then each lane walks on to its own token (consecutive tokens
@@ -151,7 +175,7 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
   uint64_t* s_full = v_free + VS;  // [2] scores of a tile
   uint64_t* p_full = s_full + 2;   // [2] its weights
   uint64_t* o_done = p_full + 2;   // [2] its product with V
-  uint64_t* turn = o_done + 2;     // [2][4] a warp's turn at the exponentials
+  uint64_t* v_clear = o_done + 2;    // the last V tile without what lies behind the prefix
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag, pos_lo, pos_hi;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -171,8 +195,8 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
       nvb::mbar_init(&s_full[q], 1);
       nvb::mbar_init(&p_full[q], 4);
       nvb::mbar_init(&o_done[q], 1);
-      for (int w = 0; w < 4; ++w) nvb::mbar_init(&turn[q * 4 + w], 1);
     }
+    nvb::mbar_init(v_clear, 1);
     nvb::fence_mbar_init();
     nvb::tma_prefetch_desc(&kmap);
     nvb::tma_prefetch_desc(&vmap);
@@ -259,6 +283,7 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
   // step j of tile q works on key tile t0 + j, or t0 + 2 j + q
   const int stride = twice ? 2 : 1;
   const int steps0 = twice ? (nt + 1) / 2 : nt, steps1 = twice ? nt / 2 : nt;
+  const bool clear = nt > 0 && (t0 + nt) * BN > kend;  // the last tile ends behind the prefix
 
   // registers: launched with 168 a thread (64512 in all); 128 * 88 + 256 * 208 is the same sum
   if (warp < 4) {
@@ -273,92 +298,88 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
       int i = early ? min(NS, nt) : 0;
       bool ok = true;
       for (; i < nt; ++i) {
-        if (i >= NS && !nvb::mbar_wait(&freeb[i % NS], ((i / NS) & 1) ^ 1, a.err, &abort_flag)) {
+        if (i >= NS && !tc_wait(&freeb[i % NS], ((i / NS) & 1) ^ 1, a.err, &abort_flag)) {
           ok = false;
           break;
         }
         copy(is_k, i);
       }
       if (!ok)  // bounded drain of copies that may still be landing
-        for (int j = (i > NS ? i - NS : 0); j < i; ++j) nvb::mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, nullptr);
+        for (int j = (i > NS ? i - NS : 0); j < i; ++j) tc_wait(&full[j % NS], (j / NS) & 1, nullptr, nullptr);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issue
-    // key tile i against Q tile q
+    // descriptors differ from these in the start address alone (16-byte units in the low bits)
+    const uint64_t q_desc = nvb::sdesc_kmajor_sw128(nvb::smem_u32(qs)), k_desc = nvb::sdesc_kmajor_sw128(nvb::smem_u32(kring));
+    const uint64_t v_desc = tc_desc_v(nvb::smem_u32(vring), C::KBOX);
+    auto wait = [&](uint64_t* bar, int phase) {
+      return __all_sync(0xffffffffu, tc_wait(bar, (uint32_t)(phase & 1), a.err, &abort_flag));
+    };
+    // scores of Q tile q against key tile i
     auto issue_s = [&](int q, int i, bool last_use) {
-      const uint32_t ka = nvb::smem_u32(kring + (size_t)(i % KS) * C::KTILE);
-      const uint32_t qa = nvb::smem_u32(qs) + (twice ? 0 : q) * C::QTILE;
+      const uint64_t kd = k_desc + (uint32_t)(i % KS) * (C::KTILE >> 4);
+      const uint64_t qd = q_desc + (uint32_t)(twice ? 0 : q) * (C::QTILE >> 4);
+      const uint32_t d = tmem + (uint32_t)q * BN;
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk)
-        nvb::tc_mma_f16(tmem + (uint32_t)q * BN, nvb::sdesc_kmajor_sw128(qa + (kk >> 2) * C::QBOX + (kk & 3) * 32),
-                        nvb::sdesc_kmajor_sw128(ka + (kk >> 2) * C::KBOX + (kk & 3) * 32), IDESC_S, kk > 0 ? 1u : 0u);
+        nvb::tc_mma_f16(d, qd + ((kk >> 2) * C::QBOX + (kk & 3) * 32) / 16,
+                  kd + ((kk >> 2) * C::KBOX + (kk & 3) * 32) / 16, IDESC_S, kk > 0 ? 1u : 0u);
       nvb::tc_commit(&s_full[q]);
       if (last_use) nvb::tc_commit(&k_free[i % KS]);
     };
     auto issue_pv = [&](int q, int i, bool first, bool last_use) {
-      const uint32_t va = nvb::smem_u32(vring + (size_t)(i % VS) * C::KTILE);
+      const uint64_t vd = v_desc + (uint32_t)(i % VS) * (C::KTILE >> 4);
+      const uint32_t d = tmem + C::O_COL + (uint32_t)q * HD, pa = tmem + (uint32_t)q * BN;
+      tc_mma_ts(d, pa, vd, IDESC_PV, first ? 0u : 1u);
 #pragma unroll
-      for (int kk = 0; kk < BN / 16; ++kk)
-        tc_mma_ts(tmem + C::O_COL + (uint32_t)q * HD, tmem + (uint32_t)q * BN + kk * 8,
-                  tc_desc_v(va + kk * 2048, C::KBOX), IDESC_PV, (!first || kk > 0) ? 1u : 0u);
+      for (int kk = 1; kk < BN / 16; ++kk) tc_mma_ts(d, pa + kk * 8, vd + kk * (2048 / 16), IDESC_PV, 1u);
       nvb::tc_commit(&o_done[q]);
       if (last_use) nvb::tc_commit(&v_free[i % VS]);
     };
-    bool ok = nt > 0;
-    for (int q = 0; ok && q < 2; ++q) {  // scores of both tiles' first steps
-      if (q == 1 && steps1 == 0) break;
-      ok = tc_handoff(1);
+    bool ok = true;
+    for (int q = 0; ok && q < (steps1 > 0 ? 2 : steps0); ++q) {  // scores of both tiles' first steps
+      const int i = twice ? q : 0;
+      ok = wait(&k_full[i % KS], i / KS);
       if (!ok) break;
       nvb::tc_fence_after();
-      if (lane == 0) issue_s(q, twice ? q : 0, twice || q == 1);
+      if (tc_elect()) issue_s(q, i, twice || q == 1);
       __syncwarp();
     }
     for (int j = 0; ok && j < steps0; ++j)
-      for (int q = 0; ok && q < 2; ++q) {
-        if (q == 1 && j >= steps1) break;
-        ok = tc_handoff(1);  // P of this step is in tensor memory, V landed; the next K tile landed
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (!ok || (q == 1 && j >= steps1)) break;
+        const int i = j * stride + (twice ? q : 0);
+        const bool more = j + 1 < (q == 0 ? steps0 : steps1);
+        // the tiles are usually there; what the issue waits for is P
+        ok = wait(i == nt - 1 && clear ? v_clear : &v_full[i % VS], i == nt - 1 && clear ? 0 : i / VS);
+        if (ok && more) ok = wait(&k_full[(i + stride) % KS], (i + stride) / KS);
+        if (ok) ok = wait(&p_full[q], j);
         if (!ok) break;
         nvb::tc_fence_after();
-        if (lane == 0) {
-          const int i = j * stride + (twice ? q : 0);
+        if (tc_elect()) {
           issue_pv(q, i, j == 0, twice || q == 1);
           // the next scores overwrite P: the tensor pipe runs MMAs in the order of issue
-          if (j + 1 < (q == 0 ? steps0 : steps1)) issue_s(q, i + stride, twice || q == 1);
+          if (more) issue_s(q, i + stride, twice || q == 1);
         }
         __syncwarp();
       }
   } else if (warp == 2) {
-    // ---------------------------------------------------------------- the issuer's waits
-    bool ok = nt > 0;
-    auto wait = [&](uint64_t* bar, int phase) {
-      int o = 1;
-      if (lane == 0) o = nvb::mbar_wait(bar, (uint32_t)(phase & 1), a.err, &abort_flag) ? 1 : 0;
-      return __shfl_sync(0xffffffffu, o, 0) != 0;
-    };
-    for (int q = 0; ok && q < 2; ++q) {
-      if (q == 1 && steps1 == 0) break;
-      const int i = twice ? q : 0;
-      ok = tc_handoff(wait(&k_full[i % KS], i / KS));
-    }
-    for (int j = 0; ok && j < steps0; ++j)
-      for (int q = 0; ok && q < 2; ++q) {
-        if (q == 1 && j >= steps1) break;
-        const int i = j * stride + (twice ? q : 0);
-        bool good = wait(&v_full[i % VS], i / VS);
-        const int tok0 = (t0 + i) * BN;
-        if (good && tok0 + BN > kend && (twice || q == 0)) {
-          // keys behind the prefix may hold anything: their weight is 0, and 0 * NaN must not reach the sum
-          uint8_t* vt = vring + (size_t)(i % VS) * C::KTILE;
-          for (int x = lane + (kend - tok0) * (HD / 8); x < BN * (HD / 8); x += 32) {
-            const int vr = x / (HD / 8), c = x % (HD / 8);
-            *reinterpret_cast<uint4*>(vt + (c >> 3) * C::KBOX + nvb::swz128(vr, c & 7)) = make_uint4(0, 0, 0, 0);
-          }
-          nvb::fence_proxy_async();
+    // ---------------------------------------------------------------- V rows behind the prefix
+    // They may hold anything: their weight is 0, and 0 * NaN must not reach the sum.
+    if (clear) {
+      const int i = nt - 1, valid = kend - (t0 + i) * BN;
+      if (__all_sync(0xffffffffu, tc_wait(&v_full[i % VS], (uint32_t)((i / VS) & 1), a.err, &abort_flag))) {
+        uint8_t* vt = vring + (size_t)(i % VS) * C::KTILE;
+        for (int x = lane + valid * (HD / 8); x < BN * (HD / 8); x += 32) {
+          const int vr = x / (HD / 8), c = x % (HD / 8);
+          *reinterpret_cast<uint4*>(vt + (c >> 3) * C::KBOX + nvb::swz128(vr, c & 7)) = make_uint4(0, 0, 0, 0);
         }
-        good = good && wait(&p_full[q], j);
-        if (j + 1 < (q == 0 ? steps0 : steps1)) good = good && wait(&k_full[(i + stride) % KS], (i + stride) / KS);
-        ok = tc_handoff(good);
+        nvb::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) nvb::mbar_arrive(v_clear);
       }
+    }
   }
   } else {
     // ---------------------------------------------------------------- softmax and output
@@ -375,18 +396,8 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
     const bool idle = !have || t >= a.T;  // nothing is written for the row: no need to mask it
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
-    // The warps of the two tiles that share an SM quarter take turns at the exponentials: left alone they run in step,
-    // and the tensor cores wait for both and then both for the tensor cores.
-    uint64_t* my_turn = &turn[tile * 4 + (warp & 3)];
-    uint64_t* other_turn = &turn[(tile ^ 1) * 4 + (warp & 3)];
     for (int j = 0; j < steps; ++j) {
-      int okw = 1;
-      if (lane == 0) {
-        okw = nvb::mbar_wait(&s_full[tile], (uint32_t)(j & 1), a.err, &abort_flag) ? 1 : 0;
-        if (tile == 1) okw = okw && nvb::mbar_wait(my_turn, (uint32_t)(j & 1), a.err, &abort_flag);
-        else if (j > 0 && j <= steps1) okw = okw && nvb::mbar_wait(my_turn, (uint32_t)((j - 1) & 1), a.err, &abort_flag);
-      }
-      if (!__shfl_sync(0xffffffffu, okw, 0)) {
+      if (!__all_sync(0xffffffffu, tc_wait(&s_full[tile], (uint32_t)(j & 1), a.err, &abort_flag))) {
         ok = false;
         break;
       }
@@ -413,68 +424,68 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
 #pragma unroll
         for (int e = 0; e < BN; ++e) u[e] = e <= hi && e > lo ? u[e] : 0xff800000u;
       }
-      float m4[4] = {val(0), val(1), val(2), val(3)};
+      // The weights are taken against the maximum in use before this tile's is known: it holds for most tiles, and the
+      // tile's own maximum is found on the way.  Where it does not (or there is none yet), once more.
+      if (!__all_sync(0xffffffffu, m_used > -INFINITY)) {
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 4; e < BN; ++e) m4[e & 3] = fmaxf(m4[e & 3], val(e));
-      const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
-      float new_m = m_used;
-      bool need = false;
-      if (mt > -INFINITY) {
-        if (m_used == -INFINITY) {
-          new_m = mt;  // the O row is still zero
-        } else if (mt > m_used + 8.f) {
-          new_m = mt;
-          need = true;
-        }
+        for (int e = 0; e < BN; e += 2) m4[(e >> 1) & 3] = fmaxf(fmaxf(val(e), val(e + 1)), m4[(e >> 1) & 3]);
+        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+        if (m_used == -INFINITY && mt > -INFINITY) m_used = mt;  // the O row is still zero
       }
-      if (__any_sync(0xffffffffu, need)) {  // j >= 1 here
-        okw = 1;
-        if (lane == 0) okw = nvb::mbar_wait(&o_done[tile], (uint32_t)((j - 1) & 1), a.err, &abort_flag) ? 1 : 0;
-        if (!__shfl_sync(0xffffffffu, okw, 0)) {
-          ok = false;
+      const uint64_t mul2 = pack2(mul, mul);
+#pragma unroll 1
+      for (int again = 0;; ++again) {
+        const float mneg = m_used == -INFINITY ? 0.f : -m_used;  // without keys every score is -inf, every weight 0
+        const uint64_t neg2 = pack2(mneg, mneg);
+        uint64_t rs0 = 0, rs1 = 0;
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t v = fma2(pack2(val(c + e), val(c + e + 1)), mul2, neg2);
+            const int pair = (e / 2) % 8;
+            float p0, p1;
+            unpack2(v, p0, p1);
+            m4[pair & 3] = fmaxf(fmaxf(p0, p1), m4[pair & 3]);
+            if (pair == 1 || pair == 4 || pair == 6) {
+              exp2_poly2(v, p0, p1);
+            } else {
+              p0 = exp2f(p0);
+              p1 = exp2f(p1);
+            }
+            if (pair & 1) rs1 = add2(rs1, pack2(p0, p1));
+            else rs0 = add2(rs0, pack2(p0, p1));
+            w[e / 2] = nvb::pack_bf16x2(p0, p1);
+          }
+          tc_st16(s_col + c / 2, w);  // over the scores, which are in registers
+        }
+        const float over = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));  // how far above the maximum in use
+        if (again > 0 || !__any_sync(0xffffffffu, over > 8.f)) {
+          float r0, r1;
+          unpack2(add2(rs0, rs1), r0, r1);
+          l += r0 + r1;
           break;
         }
-        nvb::tc_fence_after();
-        const float f = need ? exp2f(m_used - new_m) : 1.f;
+        // m_used moves: O and l follow.  Scores of this tile are there, so the product of the step before is done.
+        const float f = over > 8.f ? exp2f(-over) : 1.f;
+        if (over > 8.f) m_used += over;
         l *= f;
+        if (j > 0) {
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t u[32];
-          tc_ld32(o_col + c, u);
-          nvb::tmem_ld_wait();
-          nvb::reg_fence<32>(u);
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tc_ld32(o_col + c, o);
+            nvb::tmem_ld_wait();
+            nvb::reg_fence<32>(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
-          tc_st32(o_col + c, u);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tc_st32(o_col + c, o);
+          }
         }
-        tc_st_wait();
       }
-      m_used = new_m;
-      const float mneg = m_used == -INFINITY ? 0.f : -m_used;  // a row without keys: every score is -inf, every weight 0
-      const uint64_t mul2 = pack2(mul, mul), neg2 = pack2(mneg, mneg);
-      uint64_t rs0 = 0, rs1 = 0;
-#pragma unroll
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          float p[4];
-          unpack2(fma2(pack2(val(c + e), val(c + e + 1)), mul2, neg2), p[0], p[1]);
-          unpack2(fma2(pack2(val(c + e + 2), val(c + e + 3)), mul2, neg2), p[2], p[3]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = exp2f(p[i]);
-          rs0 = add2(rs0, pack2(p[0], p[1]));
-          rs1 = add2(rs1, pack2(p[2], p[3]));
-          w[e / 2] = nvb::pack_bf16x2(p[0], p[1]);
-          w[e / 2 + 1] = nvb::pack_bf16x2(p[2], p[3]);
-        }
-        tc_st16(s_col + c / 2, w);  // over the scores, which are in registers
-      }
-      __syncwarp();
-      if (lane == 0) nvb::mbar_arrive(other_turn);
-      float r0, r1;
-      unpack2(add2(rs0, rs1), r0, r1);
-      l += r0 + r1;
       tc_st_wait();
       nvb::tc_fence_before();
       __syncwarp();
@@ -482,7 +493,7 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
     }
     // the part: O / l and the log2-sum-exp
     int okw = ok ? 1 : 0;
-    if (ok && steps > 0 && lane == 0) okw = nvb::mbar_wait(&o_done[tile], (uint32_t)((steps - 1) & 1), a.err, &abort_flag) ? 1 : 0;
+    if (ok && steps > 0 && lane == 0) okw = tc_wait(&o_done[tile], (uint32_t)((steps - 1) & 1), a.err, &abort_flag) ? 1 : 0;
     okw = __shfl_sync(0xffffffffu, okw, 0);
     nvb::tc_fence_after();
     if (okw) {
