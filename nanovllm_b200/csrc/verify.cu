@@ -2,8 +2,8 @@
 // The reference has no counterpart; temperature, top-k and top-p mean what they mean for its sampler
 // (nano-vllm-java/src/main/java/com/igormaznitsa/nanollvm/layers/Sampler.java:69-134).
 //
-// Row r of sequence b holds the target's logits for the token after ids[r].  x = softcap(logit) (NaN counts as -inf),
-// w_i = exp((x_i - max x) / T) on the kept set S: the k largest logits (equal ones: lowest token first), of those the
+// Row r of sequence b holds the target's logits for the token after ids[r].  x = softcap(logit) (NaN counts as -inf, and
+// -inf stays -inf), w_i = exp((x_i - max x) / T) on the kept set S: the k largest logits (equal ones: lowest token first), of those the
 // shortest prefix in that order whose mass reaches top_p.  p = w / Z.  The draft d = ids[r + 1] is accepted while
 // u_r * q_d < p_d, q the distribution it was drawn from (q_d = 1 without one).  At the first refusal the next token is
 // drawn from max(0, p - q) (without q: from p without d), else from p of the sequence's last row: the first token
@@ -23,12 +23,15 @@
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int kThreads = 512;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr double kLog2e64 = 1.4426950408889634074;
-// masses are summed as integers (any order, same sum): 2^43 per unit, at most 2^20 weights of at most 1
+// masses in the radix select are integers (any order, same sum): 2^43 per unit, fewer than 2^20 weights of at most 1
 constexpr float kUnit = 8796093022208.0f;
-constexpr double kUnitInv = 1.0 / 8796093022208.0;
-constexpr int kMaxVocab = 1 << 20;
+constexpr int kMaxVocab = 327680;  // 32-bit logits of a row in the shared memory of eight CTAs
+constexpr int kMaxCluster = 8;
+constexpr int kBins = 128;   // of 1/8 octave of weight below the row's largest; the last one holds the rest
+constexpr int kList = 1024;  // tokens that a cut is found among by sorting
+constexpr float kListMargin = 1.0001f;
 
 struct VerifyArgs {
   const void* logits;
@@ -47,8 +50,9 @@ struct VerifyArgs {
   float softcap;
   int64_t* tokens;
   int* counts;
-  // per row: kept set as a composite key (logit order, then token), acceptance
+  // per row: kept set as a composite key (logit order, then token), largest logit, acceptance
   unsigned long long* cut;
+  float* row_max;
   int* accept;
   int* err;
 
@@ -58,31 +62,46 @@ struct VerifyArgs {
 };
 
 template <typename T>
-NV_DEVICE float raw_logit(const T* p, long i);
+NV_DEVICE float to_float(T v);
 template <>
-NV_DEVICE float raw_logit<float>(const float* p, long i) {
-  const float x = p[i];
-  return isnan(x) ? -INFINITY : x;
-}
+NV_DEVICE float to_float<float>(float v) { return v; }
 template <>
-NV_DEVICE float raw_logit<bf16>(const bf16* p, long i) {
-  const float x = __bfloat162float(p[i]);
-  return isnan(x) ? -INFINITY : x;
-}
+NV_DEVICE float to_float<bf16>(bf16 v) { return __bfloat162float(v); }
 NV_DEVICE uint32_t order_key(float f) {
   const uint32_t u = __float_as_uint(f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-// larger = earlier in the order "logit descending, token ascending"; -0 and +0 are one value
+NV_DEVICE float key_logit(unsigned long long k) {
+  const uint32_t u = (uint32_t)(k >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+// larger = earlier in the order "logit descending, token ascending"; NaN is -inf, -0 and +0 are one value
 NV_DEVICE unsigned long long rank_key(float x, int i) {
-  return ((unsigned long long)order_key(x + 0.f) << 32) | (0xffffffffu - (uint32_t)i);
+  return ((unsigned long long)order_key(fmaxf(x, -INFINITY) + 0.f) << 32) | (0xffffffffu - (uint32_t)i);
 }
 
-// Weights of a row relative to its largest logit.
+// 2^y for y <= 0 in 64 bits (relative error below 1e-13): y = k / 64 + r, a table of 2^(k / 64) and a polynomial for
+// 2^r, |r| <= 1/128 (the remainder of the exponential series behind the fourth power is 4e-14).
+NV_DEVICE double exp2_neg(double y, const double* table) {
+  if (!(y > -1000.0)) return 0.0;
+  const double magic = 105553116266496.0;  // 1.5 * 2^46: the last bit of y + magic is 1/64
+  const double t = y + magic;
+  const double r = y - (t - magic);
+  const int k = __double2loint(t);
+  double p = 9.618129107628477e-3;
+  p = fma(p, r, 5.550410866482158e-2);
+  p = fma(p, r, 2.402265069591007e-1);
+  p = fma(p, r, 6.931471805599453e-1);
+  p = fma(p, r, 1.0) * table[k & 63];
+  return __hiloint2double(__double2hiint(p) + (k >> 6) * (1 << 20), __double2loint(p));
+}
+
+// Weights of a row relative to its largest logit.  ``weight`` (32 bits) takes the exponent's argument as a product with
+// log2(e) / T in two floats, so that its error is the rounding of the result alone; sums of it are only used where
+// 1e-6 does not matter, or are done over in 64 bits.
 struct RowScale {
-  float m, softcap;   // largest (uncapped) logit
-  float mc;           // its capped value
-  float c_hi, c_lo;   // log2(e) / T as two floats
+  float m, softcap, mc;  // largest logit, its capped value
+  float c_hi, c_lo;      // log2(e) / T
   double m64, c64, cap64;
 
   NV_DEVICE RowScale(float m_, float cap, float T) : m(m_), softcap(cap) {
@@ -99,18 +118,38 @@ struct RowScale {
     return softcap * (1.f - 2.f / (e + 1.f));
   }
   NV_DEVICE double capped64(float x) const { return softcap > 0.f ? cap64 * tanh((double)x / cap64) : (double)x; }
-  NV_DEVICE float weight(float x) const {
-    if (x == m) return m == -INFINITY ? 0.f : 1.f;
-    const float d = capped(x) - mc;
-    if (d < -1e30f) return 0.f;  // masked (the type's lowest value, -inf) or below a +inf: no product to overflow
-    return exp2f(fminf(0.f, fmaf(d, c_hi, d * c_lo)));
+  // log2 of the weight; hugely negative for NaN, -inf and the type's lowest value (no product to overflow)
+  NV_DEVICE float log_weight(float x) const {
+    if (m == INFINITY) return x == m ? 0.f : -1e30f;
+    const float d = softcap > 0.f && x == -INFINITY ? -1e30f : fmaxf(capped(x) - mc, -1e30f);
+    return fminf(0.f, fmaf(d, c_hi, d * c_lo));
   }
-  NV_DEVICE double weight64(float x) const {
+  NV_DEVICE float weight(float x) const { return exp2f(log_weight(x)); }
+  NV_DEVICE double weight64(float x, const double* table) const {
     if (x == m) return m == -INFINITY ? 0.0 : 1.0;
-    const double d = capped64(x) - m64;
-    return d < -1e30 ? 0.0 : exp2(d * c64);
+    const double d = x == -INFINITY ? -1e300 : capped64(x) - m64;  // masked stays masked, also under a soft-cap
+    return d > -1e30 ? exp2_neg(fmin(0.0, d * c64), table) : 0.0;  // NaN: 0
   }
 };
+
+NV_DEVICE uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+template <typename T>
+NV_DEVICE T peer_load(const T* p, uint32_t rank) {  // the same variable of another CTA of the cluster
+  const uint32_t at = nvb::map_peer(nvb::smem_u32(p), rank);
+  if constexpr (sizeof(T) == 8) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+    return *reinterpret_cast<T*>(&v);
+  } else {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return *reinterpret_cast<T*>(&v);
+  }
+}
 
 template <typename T>
 NV_DEVICE T block_sum(T v, T* sh) {
@@ -120,16 +159,45 @@ NV_DEVICE T block_sum(T v, T* sh) {
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
   T r = sh[0];
-  for (int i = 1; i < kThreads / 32; ++i) r += sh[i];
+  for (int i = 1; i < kWarps; ++i) r += sh[i];
   return r;
 }
+// Sum over the cluster, the same in every thread.  ``slot``: one for each call of a kernel.
+template <typename T>
+NV_DEVICE T cluster_sum(T v, T* sh, T* slot) {
+  v = block_sum(v, sh);
+  const uint32_t n = cluster_size();
+  if (n == 1) return v;
+  if (threadIdx.x == 0) *slot = v;
+  nvb::cluster_sync();
+  T r = peer_load(slot, 0);
+  for (uint32_t i = 1; i < n; ++i) r += peer_load(slot, i);
+  return r;
+}
+NV_DEVICE float cluster_max(float v, float* sh, float* slot) {
+  v = nvb::warp_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) v = fmaxf(v, sh[i]);
+  const uint32_t n = cluster_size();
+  if (n == 1) return v;
+  if (threadIdx.x == 0) *slot = v;
+  nvb::cluster_sync();
+  for (uint32_t i = 0; i < n; ++i) v = fmaxf(v, peer_load(slot, i));
+  return v;
+}
 
+// Sequence of row r by a 32-way search of the warp: the last b with cu_q[b] <= r.
 NV_DEVICE int seq_of_row(const int* cu_q, int B, int r) {
-  int lo = 0, hi = B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu_q[mid] <= r) lo = mid;
-    else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, len = B;
+  while (len > 1) {
+    const int step = (len + 31) / 32, at = lo + lane * step;
+    const bool below = at < lo + len && cu_q[at] <= r;
+    const int skip = max(0, __popc(__ballot_sync(0xffffffffu, below)) - 1) * step;
+    lo += skip;
+    len = min(step, len - skip);
   }
   return lo;
 }
@@ -147,196 +215,566 @@ NV_DEVICE int draft_row(const VerifyArgs& a, int b, int r, int* sh) {
   return r - block_sum(nonempty, sh);
 }
 
-// One CTA per row: the kept set and, where the row holds a draft, its acceptance.
+// This CTA's part of a row in shared memory: tokens [lo, hi) of it, at the same offset in their 16 bytes as in global
+// memory, so that whole words come by one asynchronous copy; what the first and last word hold besides is -inf.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(VerifyArgs a) {
-  nvb::pdl_wait();
-  nvb::pdl_trigger();
-  __shared__ unsigned long long hist[256], sh_u[32];
-  __shared__ float sh_f[32];
-  __shared__ int sh_i[32];
-  __shared__ unsigned long long sel_prefix, sel_before;
-  const int r = blockIdx.x, tid = threadIdx.x, V = a.V;
-  const int b = seq_of_row(a.cu_q, a.B, r);
-  const int2 rows = seq_rows(a, b);
-  if (r < rows.x || r >= rows.y) return;
-  const T* x = reinterpret_cast<const T*>(a.logits) + r * a.ld;
-  float m = -INFINITY;
-  for (int i = tid; i < V; i += kThreads) m = fmaxf(m, raw_logit(x, i));
-  m = nvb::warp_max(m);
-  if ((tid & 31) == 0) sh_f[tid >> 5] = m;
+struct Slice {
+  static constexpr int PER = 16 / sizeof(T);
+  const T* words;  // 16-byte aligned
+  int lo, hi, nw, first;  // token of word w, element e: first + w * PER + e
+
+  template <typename F>
+  NV_DEVICE void each(int w, F f) const {
+    const uint4 v = reinterpret_cast<const uint4*>(words)[w];
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) f(to_float(e[j]), first + w * PER + j);
+  }
+};
+
+NV_DEVICE int slice_tokens(int V, int n) { return ((V + n - 1) / n + 7) / 8 * 8; }
+
+template <typename T>
+NV_DEVICE Slice<T> load_slice(const T* row, int V, uint8_t* buf, uint64_t* bar, int* err) {
+  Slice<T> s;
+  const int per = slice_tokens(V, cluster_size()), tid = threadIdx.x;
+  s.lo = min(V, (int)nvb::cluster_ctarank() * per);
+  s.hi = min(V, s.lo + per);
+  const uintptr_t g0 = reinterpret_cast<uintptr_t>(row + s.lo), g1 = reinterpret_cast<uintptr_t>(row + s.hi);
+  const int off = (int)(g0 & 15);
+  s.words = reinterpret_cast<const T*>(buf);
+  s.first = s.lo - off / (int)sizeof(T);
+  s.nw = (off + (int)(g1 - g0) + 15) / 16;
+  const uintptr_t a0 = (g0 + 15) & ~uintptr_t(15), a1 = g1 & ~uintptr_t(15);
+  const bool bulk = a1 > a0;
+  if (tid == 0) {
+    nvb::mbar_init(bar, 1);
+    nvb::fence_mbar_init();
+    if (bulk) {
+      const uint32_t bytes = (uint32_t)(a1 - a0);
+      nvb::mbar_arrive_expect_tx(bar, bytes);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       nvb::smem_u32(buf + off + (a0 - g0))),
+                   "l"(a0), "r"(bytes), "r"(nvb::smem_u32(bar))
+                   : "memory");
+    }
+  }
+  // the ends of the first and last word
+  const int n_head = bulk ? (int)(a0 - g0) / (int)sizeof(T) : s.hi - s.lo;
+  const int n_tail = bulk ? (int)(g1 - a1) / (int)sizeof(T) : 0;
+  T* el = reinterpret_cast<T*>(buf);
+  const int skip = off / (int)sizeof(T), n = s.hi - s.lo;
+  if (tid < skip) el[tid] = (T)(-INFINITY);
+  if (tid < n_head) el[skip + tid] = row[s.lo + tid];
+  if (tid < n_tail) el[skip + n - n_tail + tid] = row[s.hi - n_tail + tid];
+  for (int i = skip + n + tid; i < s.nw * Slice<T>::PER; i += kThreads) el[i] = (T)(-INFINITY);
   __syncthreads();
-  for (int i = 0; i < kThreads / 32; ++i) m = fmaxf(m, sh_f[i]);
-  const RowScale rs(m, a.softcap, a.temps[b]);
-  // radix select over the composite keys, 8 bits a pass: the smallest kept key when weights (1 or mass) are summed in
-  // descending key order up to ``target``; of the keys >= floor_key
-  auto select = [&](bool by_mass, unsigned long long target, unsigned long long floor_key) {
-    unsigned long long prefix = 0, mask = 0, before = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < V; i += kThreads) {
-        const float xv = raw_logit(x, i);
-        const unsigned long long k = rank_key(xv, i);
-        if (k >= floor_key && (k & mask) == prefix)
-          atomicAdd(&hist[(k >> shift) & 255], by_mass ? (unsigned long long)(rs.weight(xv) * kUnit) : 1ull);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        unsigned long long cum = before;
-        int bin = 255;
-        for (; bin > 0; --bin) {
-          if (cum + hist[bin] >= target) break;
-          cum += hist[bin];
-        }
-        sel_prefix = prefix | ((unsigned long long)bin << shift);
-        sel_before = cum;
-      }
-      __syncthreads();
-      prefix = sel_prefix;
-      before = sel_before;
-      mask |= 255ull << shift;
-      __syncthreads();
-    }
-    return prefix;
-  };
-  auto mass_from = [&](unsigned long long floor_key) {
-    unsigned long long z = 0;
-    for (int i = tid; i < V; i += kThreads) {
-      const float xv = raw_logit(x, i);
-      if (rank_key(xv, i) >= floor_key) z += (unsigned long long)(rs.weight(xv) * kUnit);
-    }
-    return block_sum(z, sh_u);
-  };
-  const int k = a.topk[b];
-  const float top = a.topp[b];
-  unsigned long long cut = 0;
-  if (k > 0 && k < V) cut = select(false, (unsigned long long)k, 0);
-  if (top < 1.f && m != -INFINITY) {
-    const double P = (double)mass_from(cut) * (double)top;
-    const unsigned long long target = P > 1.0 ? (unsigned long long)ceil(P) : 1ull;  // the first token always stays
-    cut = max(cut, select(true, target, cut));
-  }
-  if (tid == 0) a.cut[r] = cut;
-  if (r + 1 == rows.y) return;  // no draft after the last row
-  const long d = a.ids[r + 1];
-  const int dr = a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
-  if (a.probs != nullptr && dr >= a.D) {
-    if (tid == 0) nvb::record_error(a.err, nvb::kErrBadArgument);
-    if (tid == 0) a.accept[r] = 0;
-    return;
-  }
-  const unsigned long long z = mass_from(cut);
-  double w = 0.0, uq = 0.0;
-  if (d >= 0 && d < V) {
-    const float xv = raw_logit(x, d);
-    if (rank_key(xv, (int)d) >= cut) w = rs.weight64(xv);
-    uq = a.uniform(r) * (a.probs != nullptr ? (double)a.probs[dr * a.probs_ld + d] : 1.0);
-  }
-  double Z = (double)z * kUnitInv;
-  if (fabs(uq * Z - w) <= 1e-4 * w) {  // too near for the 32-bit weights: sum the row in 64 bits
-    double z64 = 0.0;
-    for (int i = tid; i < V; i += kThreads) {
-      const float xv = raw_logit(x, i);
-      if (rank_key(xv, i) >= cut) z64 += rs.weight64(xv);
-    }
-    Z = block_sum(z64, reinterpret_cast<double*>(sh_u));
-  }
-  if (tid == 0) a.accept[r] = uq * Z < w;
+  if (bulk) nvb::mbar_wait(bar, 0, err, nullptr);
+  return s;
 }
 
-// One CTA per sequence: the accepted drafts and the drawn token.
+NV_DEVICE void fill_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x / 64.0);
+}
+
+// One cluster per row: the kept set and, where the row holds a draft, its acceptance.  The row stays in the cluster's
+// shared memory, every pass after the load reads it there; bound by the bytes of the logits.
+//   no cut     maximum, sum of the weights
+//   top_k 1    maximum, its lowest token
+//   cuts       counts by 1/8 octave of weight bound where the cut falls; the tokens above that (and one bin more, so
+//              that roundings of the weight do not matter) are sorted when they are few, else the tokens of the bins in
+//              question go through a radix select over composite keys
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs a) {
   nvb::pdl_wait();
   nvb::pdl_trigger();
-  __shared__ double sh_d[32];
-  __shared__ int sh_i[32], sh_tok;
-  __shared__ float sh_f[32];
-  const int b = blockIdx.x, tid = threadIdx.x, V = a.V, lane = tid & 31, warp = tid >> 5;
+  extern __shared__ __align__(128) uint8_t buf[];
+  __shared__ uint64_t bar;
+  __shared__ float sh_f[32], slot_f;
+  __shared__ double sh_d[32], slot_d[3], table[64];
+  __shared__ int sh_i[32];
+  __shared__ unsigned long long sh_u[32], slot_u[2];
+  __shared__ unsigned int hist[kBins], hist_all[kBins];
+  __shared__ unsigned long long hist_m[2][256];
+  __shared__ unsigned long long keys[kList];
+  __shared__ unsigned int n_list, slot_n;
+  __shared__ int sel[4];
+  __shared__ unsigned long long sel_u[2], cut_sh;
+  __shared__ double z_sh;
+  const int r = blockIdx.x / cluster_size(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
+  const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
+  const int b = seq_of_row(a.cu_q, a.B, r);
+  const int2 rows = seq_rows(a, b);
+  if (r < rows.x || r >= rows.y) return;  // the whole cluster
+  fill_table(table);
+  if (tid < kBins) hist[tid] = 0;
+  if (tid == 0) n_list = 0;
+  const T* x = reinterpret_cast<const T*>(a.logits) + r * a.ld;
+  const Slice<T> s = load_slice(x, V, buf, &bar, a.err);
+  float m = -INFINITY;
+  for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { m = fmaxf(m, v); });
+  m = cluster_max(m, sh_f, &slot_f);
+  const RowScale rs(m, a.softcap, a.temps[b]);
+  const int k = a.topk[b];
+  const float top = a.topp[b];
+  const bool cut_k = k > 0 && k < V, cut_p = top < 1.f;
+  unsigned long long cut = 0;
+  double Z = 0.0;
+  if (k == 1) {
+    // the lowest token among the largest logits
+    unsigned long long best = 0;
+    for (int w = tid; w < s.nw; w += kThreads)
+      s.each(w, [&](float v, int i) {
+        if (v == m) best = max(best, rank_key(v, i));
+      });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) sh_u[warp] = best;
+    __syncthreads();
+    for (int i = 0; i < kWarps; ++i) best = max(best, sh_u[i]);
+    if (CL > 1) {
+      if (tid == 0) slot_u[0] = best;
+      nvb::cluster_sync();
+      for (uint32_t i = 0; i < CL; ++i) best = max(best, peer_load(&slot_u[0], i));
+    }
+    cut = m == -INFINITY ? 0 : best;
+    Z = 1.0;
+  } else {
+    const bool cuts = (cut_k || cut_p) && m != -INFINITY;
+    float z4[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int w = tid; w < s.nw; w += kThreads) {
+      int j = 0;
+      s.each(w, [&](float v, int) {
+        const float lw = rs.log_weight(v);
+        z4[j++ & 3] += exp2f(lw);
+        if (cuts) {
+          const int bin = (int)fminf(lw * -8.f, (float)(kBins - 1));
+          if (bin < kBins - 1) atomicAdd(&hist[bin], 1u);
+        }
+      });
+    }
+    Z = cluster_sum((double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]), sh_d, &slot_d[0]);
+    if (cuts) {
+      // counts of the whole row (the sum above was a barrier of the cluster, or of the only CTA)
+      if (tid < kBins - 1) {
+        unsigned int n = 0;
+        for (uint32_t i = 0; i < CL; ++i) n += CL > 1 ? peer_load(&hist[tid], i) : hist[tid];
+        hist_all[tid] = n;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        // lane: 4 bins.  lowest and highest mass that the counts allow, from the largest weights on
+        unsigned int cnt = 0;
+        float low = 0.f, high = 0.f;
+        unsigned int c4[4];
+        float l4[4], h4[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int bin = lane * 4 + j;
+          const unsigned int n = bin < kBins - 1 ? hist_all[bin] : 0u;
+          c4[j] = cnt += n;
+          l4[j] = low += n * exp2f((bin + 1.01f) * -0.125f);
+          h4[j] = high += n * exp2f((bin - 0.01f) * -0.125f);
+        }
+        unsigned int ci = cnt;
+        float li = low, hi = high;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned int cu = __shfl_up_sync(0xffffffffu, ci, o);
+          const float lu = __shfl_up_sync(0xffffffffu, li, o), hu = __shfl_up_sync(0xffffffffu, hi, o);
+          if (lane >= o) ci += cu, li += lu, hi += hu;
+        }
+        const float want = (float)((double)top * Z);
+        // first bin that certainly / possibly reaches the target
+        int sure_k = kBins - 1, sure_p = kBins - 1, may_p = kBins - 1;
+#pragma unroll
+        for (int j = 3; j >= 0; --j) {
+          const int bin = lane * 4 + j;
+          if (bin >= kBins - 1) continue;
+          if (ci - cnt + c4[j] >= (unsigned int)k) sure_k = bin;
+          if (li - low + l4[j] >= want * kListMargin) sure_p = bin;
+          if (hi - high + h4[j] >= want / kListMargin) may_p = bin;
+        }
+        sure_k = __reduce_min_sync(0xffffffffu, sure_k);
+        sure_p = __reduce_min_sync(0xffffffffu, sure_p);
+        may_p = __reduce_min_sync(0xffffffffu, may_p);
+        if (lane == 0) {
+          sel[0] = sure_k;
+          sel[1] = sure_p;
+          sel[2] = may_p;
+        }
+        // tokens up to the bin after the one that certainly holds the cut
+        const int need = min(kBins - 1, (cut_k ? sure_k : sure_p) + 1);
+        unsigned int at = need < kBins - 1 && (cut_k ? sure_k : sure_p) < kBins - 1 ? 0u : 0xffffffffu;
+        if (at == 0u) {
+          const unsigned int upto = __shfl_sync(0xffffffffu, ci - cnt, need / 4);
+          unsigned int in4 = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j == need % 4) in4 = c4[j];
+          at = upto + __shfl_sync(0xffffffffu, in4, need / 4);
+        }
+        if (lane == 0) sel[3] = at <= (unsigned int)kList ? need : -1;
+      }
+      __syncthreads();
+      const int last_bin = sel[3];
+      if (last_bin >= 0) {
+        // ------------------------------------------------ few tokens: collect, sort, walk
+        for (int w = tid; w < s.nw; w += kThreads)
+          s.each(w, [&](float v, int i) {
+            if ((int)fminf(rs.log_weight(v) * -8.f, (float)(kBins - 1)) <= last_bin)
+              keys[atomicAdd(&n_list, 1u)] = rank_key(v, i);
+          });
+        __syncthreads();
+        const unsigned int mine = n_list;
+        if (CL > 1) {
+          nvb::cluster_sync();
+          if (rank == 0) {  // gather behind the own ones
+            unsigned int at = mine;
+            for (uint32_t q = 1; q < CL; ++q) {
+              const unsigned int n = peer_load(&n_list, q);
+              for (unsigned int i = tid; i < n; i += kThreads) keys[at + i] = peer_load(&keys[i], q);
+              at += n;
+            }
+            if (tid == 0) slot_n = at;
+          }
+        } else if (tid == 0) {
+          slot_n = mine;
+        }
+        __syncthreads();
+        if (rank == 0) {
+          const int n = (int)slot_n;
+          int n2 = 32;
+          while (n2 < n) n2 *= 2;
+          for (int i = n + tid; i < n2; i += kThreads) keys[i] = 0;
+          __syncthreads();
+          for (int size = 2; size <= n2; size *= 2)
+            for (int d = size / 2; d > 0; d /= 2) {
+              for (int i = tid; i < n2 / 2; i += kThreads) {
+                const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
+                const bool down = (lo & size) == 0;
+                const unsigned long long p = keys[lo], q = keys[hi];
+                if ((p < q) == down) {
+                  keys[lo] = q;
+                  keys[hi] = p;
+                }
+              }
+              __syncthreads();
+            }
+          // weights in order, two tokens per thread, and the sums before each
+          const int nk = cut_k ? min(k, n) : n;
+          double w2[2], sum = 0.0;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int i = tid * 2 + j;
+            w2[j] = i < nk ? rs.weight64(key_logit(keys[i]), table) : 0.0;
+            sum += w2[j];
+          }
+          double incl = sum;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+          }
+          if (lane == 31) sh_d[warp] = incl;
+          __syncthreads();
+          double base = 0.0, all = 0.0;
+          for (int i = 0; i < kWarps; ++i) {
+            if (i < warp) base += sh_d[i];
+            all += sh_d[i];
+          }
+          const double want = cut_p ? (double)top * (cut_k ? all : Z) : 4.0 * kMaxVocab;
+          double before = base + incl - sum, kept = 0.0;
+          int last = -1;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int i = tid * 2 + j;
+            if (i < nk && (i == 0 || before < want)) {
+              last = i;
+              kept += w2[j];
+            }
+            before += w2[j];
+          }
+          last = __reduce_max_sync(0xffffffffu, last);
+          if (lane == 0) sh_i[warp] = last;
+          kept = block_sum(kept, sh_d);
+          for (int i = 0; i < kWarps; ++i) last = max(last, sh_i[i]);
+          if (tid == 0) {
+            cut_sh = keys[last];
+            z_sh = kept;
+          }
+          __syncthreads();
+          cut = cut_sh;
+          Z = z_sh;
+        }
+      } else {
+        // ------------------------------------------------ many: radix select, 8 bits a pass, over the tokens of bins
+        // [from, upto]; all tokens of the bins before are kept
+        auto bin_of = [&](float v) { return (int)fminf(rs.log_weight(v) * -8.f, (float)(kBins - 1)); };
+        int flip = 0;
+        auto select = [&](bool by_mass, unsigned long long target, unsigned long long before, int from, int upto,
+                          unsigned long long floor_key) {
+          unsigned long long prefix = 0, mask = 0;
+          for (int shift = 56; shift >= 0; shift -= 8) {
+            unsigned long long* h = hist_m[flip];
+            for (int i = tid; i < 256; i += kThreads) h[i] = 0;
+            __syncthreads();
+            for (int w = tid; w < s.nw; w += kThreads)
+              s.each(w, [&](float v, int i) {
+                const int bin = bin_of(v);
+                const unsigned long long key = rank_key(v, i);
+                if (bin >= from && bin <= upto && key >= floor_key && (key & mask) == prefix && i >= s.lo && i < s.hi)
+                  atomicAdd(&h[(key >> shift) & 255], by_mass ? (unsigned long long)(rs.weight(v) * kUnit) : 1ull);
+              });
+            __syncthreads();
+            if (CL > 1) nvb::cluster_sync();
+            // every CTA adds up the cluster's bins and finds the same one
+            if (tid < 256) {
+              unsigned long long v = 0;
+              for (uint32_t i = 0; i < CL; ++i) v += CL > 1 ? peer_load(&h[tid], i) : h[tid];
+              keys[tid] = v;
+            }
+            __syncthreads();
+            if (warp == 0) {  // lane: 8 bins from the top
+              unsigned long long own = 0;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) own += keys[255 - lane * 8 - i];
+              unsigned long long incl = own;
+#pragma unroll
+              for (int o = 1; o < 32; o <<= 1) {
+                const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+              }
+              const unsigned hit = __ballot_sync(0xffffffffu, before + incl >= target);
+              if (lane == (hit != 0 ? __ffs(hit) - 1 : 31)) {
+                unsigned long long cum = before + incl - own;
+                int bin = 255 - lane * 8;
+                for (; bin > 248 - lane * 8 && cum + keys[bin] < target; --bin) cum += keys[bin];
+                sel_u[0] = prefix | ((unsigned long long)bin << shift);
+                sel_u[1] = cum;
+              }
+            }
+            __syncthreads();
+            prefix = sel_u[0];
+            before = sel_u[1];
+            mask |= 255ull << shift;
+            flip ^= 1;  // the peers may still read the other one
+            __syncthreads();
+          }
+          return prefix;
+        };
+        auto count_before = [&](int from) {
+          unsigned long long n = 0;
+          for (int i = 0; i < from; ++i) n += hist_all[i];
+          return n;
+        };
+        auto mass_of = [&](int upto, unsigned long long floor_key, unsigned long long* slot) {
+          unsigned long long z = 0;
+          for (int w = tid; w < s.nw; w += kThreads)
+            s.each(w, [&](float v, int i) {
+              if (bin_of(v) <= upto && rank_key(v, i) >= floor_key) z += (unsigned long long)(rs.weight(v) * kUnit);
+            });
+          return cluster_sum(z, sh_u, slot);
+        };
+        if (cut_k) {
+          const int from = max(0, sel[0] - 1);
+          cut = select(false, (unsigned long long)k, count_before(from), from, min(kBins - 1, sel[0] + 1), 0);
+        }
+        if (cut_p) {
+          unsigned long long total = mass_of(kBins, cut, &slot_u[0]);
+          const double want = (double)total * (double)top;
+          const unsigned long long target = want > 1.0 ? (unsigned long long)ceil(want) : 1ull;  // the first always stays
+          const int from = cut_k ? 0 : max(0, sel[2] - 1), upto = cut_k ? kBins - 1 : min(kBins - 1, sel[1] + 1);
+          const unsigned long long before = from > 0 ? mass_of(from - 1, cut, &slot_u[1]) : 0ull;
+          cut = max(cut, select(true, target, before, from, upto, cut));
+        }
+        double z = 0.0;
+        for (int w = tid; w < s.nw; w += kThreads) {
+          float part = 0.f;
+          s.each(w, [&](float v, int i) {
+            if (rank_key(v, i) >= cut) part += rs.weight(v);
+          });
+          z += part;
+        }
+        Z = cluster_sum(z, sh_d, &slot_d[1]);
+      }
+    }
+  }
+  if (rank == 0 && tid == 0) {
+    a.cut[r] = cut;
+    a.row_max[r] = m;
+  }
+  if (r + 1 < rows.y) {  // the draft
+    bool near = false;
+    double w = 0.0, uq = 0.0;
+    if (rank == 0) {
+      const int dr = a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
+      const long d = a.ids[r + 1];
+      if (a.probs != nullptr && dr >= a.D) {
+        if (tid == 0) nvb::record_error(a.err, nvb::kErrBadArgument);
+      } else if (d >= 0 && d < V) {
+        const float v = to_float(x[d]);
+        if (rank_key(v, (int)d) >= cut) w = rs.weight64(v, table);
+        uq = a.uniform(r) * (a.probs != nullptr ? (double)a.probs[dr * a.probs_ld + d] : 1.0);
+      }
+      near = fabs(uq * Z - w) <= 1e-4 * w;  // too near for a sum of 32-bit weights
+      if (tid == 0) sel[0] = near;
+    }
+    if (CL > 1) {
+      nvb::cluster_sync();
+      near = peer_load(&sel[0], 0) != 0;
+      if (near) cut = rank == 0 ? cut : 0;  // only rank 0 needs to know the cut from here
+    }
+    if (near) {
+      if (CL > 1) {
+        if (rank == 0 && tid == 0) sel_u[0] = cut;
+        nvb::cluster_sync();
+        cut = peer_load(&sel_u[0], 0);
+      }
+      double z64 = 0.0;
+      for (int q = tid; q < s.nw; q += kThreads)
+        s.each(q, [&](float v, int i) {
+          if (rank_key(v, i) >= cut && i >= s.lo && i < s.hi) z64 += rs.weight64(v, table);
+        });
+      Z = cluster_sum(z64, sh_d, &slot_d[2]);
+    }
+    if (rank == 0 && tid == 0) a.accept[r] = uq * Z < w;
+  }
+  if (CL > 1) nvb::cluster_sync();  // nobody leaves while its shared memory may be read
+}
+
+// One cluster per sequence: the accepted drafts and the drawn token.  Weights and sums in 64 bits: the token depends on
+// which side of a sum the uniform falls, and a row has as many sums as tokens.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs a) {
+  nvb::pdl_wait();
+  nvb::pdl_trigger();
+  extern __shared__ __align__(128) uint8_t buf[];
+  __shared__ uint64_t bar;
+  __shared__ double sh_d[32], slot_d, table[64], warp_sum_sh[2][kWarps], all_sh[kMaxCluster * kWarps + 1];
+  __shared__ int sh_i[32];
+  const int b = blockIdx.x / cluster_size(), tid = threadIdx.x, V = a.V, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
   const int2 rows = seq_rows(a, b);
   const int n = rows.y - rows.x;
-  if (n <= 0) {
-    for (int j = tid; j < a.max_q; j += kThreads) a.tokens[(long)b * a.max_q + j] = -1;
-    if (tid == 0) {
-      a.counts[b] = 0;
-      if (n < 0) nvb::record_error(a.err, nvb::kErrBadArgument);
+  int64_t* out = a.tokens + (long)b * a.max_q;
+  if (n <= 0) {  // the whole cluster
+    if (rank == 0) {
+      for (int j = tid; j < a.max_q; j += kThreads) out[j] = -1;
+      if (tid == 0) {
+        a.counts[b] = 0;
+        if (n < 0) nvb::record_error(a.err, nvb::kErrBadArgument);
+      }
     }
     return;
   }
-  int acc = 0;
-  while (acc < n - 1 && a.accept[rows.x + acc]) ++acc;
+  fill_table(table);
+  int acc = n - 1;  // accepted drafts: up to the first refusal
+  for (int j0 = 0; j0 < n - 1; j0 += 32) {
+    const bool no = j0 + lane < n - 1 && !a.accept[rows.x + j0 + lane];
+    const unsigned refused = __ballot_sync(0xffffffffu, no);
+    if (refused != 0) {
+      acc = j0 + __ffs(refused) - 1;
+      break;
+    }
+  }
   const int r = rows.x + acc;
   const bool rejected = acc < n - 1;
-  const T* x = reinterpret_cast<const T*>(a.logits) + r * a.ld;
+  const Slice<T> s = load_slice(reinterpret_cast<const T*>(a.logits) + r * a.ld, V, buf, &bar, a.err);
   const unsigned long long cut = a.cut[r];
-  float m = -INFINITY;
-  for (int i = tid; i < V; i += kThreads) m = fmaxf(m, raw_logit(x, i));
-  m = nvb::warp_max(m);
-  if (lane == 0) sh_f[warp] = m;
-  __syncthreads();
-  for (int i = 0; i < kThreads / 32; ++i) m = fmaxf(m, sh_f[i]);
-  const RowScale rs(m, a.softcap, a.temps[b]);
-  auto weight = [&](int i) {
-    const float xv = raw_logit(x, i);
-    return rank_key(xv, i) >= cut ? rs.weight64(xv) : 0.0;
-  };
-  double z = 0.0;
-  for (int i = tid; i < V; i += kThreads) z += weight(i);
-  const double Z = block_sum(z, sh_d);
+  const RowScale rs(a.row_max[r], a.softcap, a.temps[b]);
   const int dr = rejected && a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
   const float* q = rejected && a.probs != nullptr && dr < a.D ? a.probs + dr * a.probs_ld : nullptr;
   const long drafted = rejected && a.probs == nullptr ? a.ids[r + 1] : -1;
-  const int chunk = (V + kThreads - 1) / kThreads, c0 = min(V, tid * chunk), c1 = min(V, c0 + chunk);
+  auto weight = [&](float v, int i) { return rank_key(v, i) >= cut && i >= s.lo && i < s.hi ? rs.weight64(v, table) : 0.0; };
+  double Zinv = 1.0;
+  if (q != nullptr) {  // p - q needs p itself
+    double z = 0.0;
+    for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int i) { z += weight(v, i); });
+    const double Z = cluster_sum(z, sh_d, &slot_d);
+    Zinv = Z > 0.0 ? 1.0 / Z : 0.0;
+  }
+  // warps own consecutive words, lanes one word at a time
+  const int per = (s.nw + kWarps - 1) / kWarps, w0 = min(s.nw, warp * per), w1 = min(s.nw, w0 + per);
   for (int plain = rejected ? 0 : 1; plain < 2; ++plain) {
     // plain: the probabilities themselves (also when nothing is left of p - q)
-    auto left = [&](int i) {
-      const double w = weight(i);
+    auto left = [&](float v, int i) {
+      const double w = weight(v, i);
       if (plain || w == 0.0) return w;
-      if (q != nullptr) return fmax(0.0, w / Z - (double)q[i]);
+      if (q != nullptr) return fmax(0.0, w * Zinv - (double)q[i]);
       return i == drafted ? 0.0 : w;
     };
-    double s = 0.0;
-    for (int i = c0; i < c1; ++i) s += left(i);
-    double incl = s;
+    double sum = 0.0;
+    for (int w = w0 + lane; w < w1; w += 32) s.each(w, [&](float v, int i) { sum += left(v, i); });
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) warp_sum_sh[plain][warp] = sum;
+    __syncthreads();
+    if (CL > 1) nvb::cluster_sync();
+    // sums before each warp of the cluster, in token order; every CTA computes the same ones
+    const int nws = (int)CL * kWarps;
+    if (tid < nws) all_sh[tid] = CL > 1 ? peer_load(&warp_sum_sh[plain][tid % kWarps], tid / kWarps) : warp_sum_sh[plain][tid];
+    __syncthreads();
+    if (tid == 0) {
+      double c = 0.0;  // one after the other: the sums never decrease
+      for (int i = 0; i < nws; i += kWarps) {
+        double v[kWarps];
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) v[k] = all_sh[i + k];
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          all_sh[i + k] = c;
+          c += v[k];
+        }
+      }
+      all_sh[nws] = c;
     }
     __syncthreads();
-    if (lane == 31) sh_d[warp] = incl;
-    if (tid == 0) sh_tok = 0x7fffffff;
-    __syncthreads();
-    double base = 0.0, total = 0.0;
-    for (int i = 0; i < kThreads / 32; ++i) {
-      if (i < warp) base += sh_d[i];
-      total += sh_d[i];
-    }
+    const double total = all_sh[nws];
     if (total > 0.0) {
       // below total whatever the uniform is, so some token exceeds it
       const double want = fmin(fmax(a.uniform(rows.y - 1), 0.0), 1.0 - 2.220446049250313e-16) * total;
-      double c = base + incl - s;
-      if (s > 0.0 && base + incl > want) {
+      const int me = (int)rank * kWarps + warp;
+      double c = all_sh[me];
+      if (c <= want && all_sh[me + 1] > want) {  // this warp's words hold it
         int tok = -1;
-        for (int i = c0; i < c1; ++i) {
-          const double v = left(i);
-          c += v;
-          if (v > 0.0) tok = i;
-          if (v > 0.0 && c > want) break;
+        for (int wb = w0; wb < w1; wb += 32) {
+          double mine = 0.0;
+          if (wb + lane < w1) s.each(wb + lane, [&](float v, int i) { mine += left(v, i); });
+          double incl = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+          }
+          const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && c + incl > want);
+          const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
+          const int src = over != 0 ? __ffs(over) - 1 : some != 0 ? 31 - __clz(some) : -1;
+          int cand = -1;
+          if (lane == src) {
+            double d = c + incl - mine;
+            s.each(wb + lane, [&](float v, int i) {
+              const double l = left(v, i);
+              if (l > 0.0 && !(cand >= 0 && d > want)) cand = i;
+              d += l;
+            });
+          }
+          if (src >= 0) tok = __shfl_sync(0xffffffffu, cand, src);
+          if (over != 0) break;
+          c += __shfl_sync(0xffffffffu, incl, 31);
         }
-        atomicMin(&sh_tok, tok);
+        if (lane == 0) out[acc] = tok < 0 ? 0 : tok;
       }
+      break;
     }
-    __syncthreads();
-    if (total > 0.0) break;
+    if (plain == 1 && rank == 0 && tid == 0) out[acc] = 0;  // no logit above -inf
   }
-  if (tid == 0) {
-    int64_t* out = a.tokens + (long)b * a.max_q;
-    for (int j = 0; j < a.max_q; ++j) out[j] = j < acc ? a.ids[rows.x + j + 1] : -1;
-    out[acc] = sh_tok == 0x7fffffff ? 0 : sh_tok;
-    a.counts[b] = acc + 1;
+  if (rank == 0) {
+    for (int j = tid; j < a.max_q; j += kThreads)
+      if (j != acc) out[j] = j < acc ? a.ids[rows.x + j + 1] : -1;
+    if (tid == 0) a.counts[b] = acc + 1;
   }
+  if (CL > 1) nvb::cluster_sync();  // nobody leaves while its shared memory may be read
 }
 
 }  // namespace
@@ -350,7 +788,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
                   (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
               "logits must be bf16 or fp32 [rows, vocabulary]");
   const int64_t R = logits.size(0), V = logits.size(1), B = cu_q.numel() - 1;
-  TORCH_CHECK(V >= 1 && V <= kMaxVocab, "the vocabulary must have 1 to 1048576 tokens");
+  TORCH_CHECK(V >= 1 && V <= kMaxVocab, "the vocabulary must have 1 to 327680 tokens");
   TORCH_CHECK(R == 0 || V == 1 || logits.stride(1) == 1, "logits rows must be contiguous");
   auto vec = [&](const at::Tensor& t, at::ScalarType type, int64_t n, const char* what) {
     TORCH_CHECK(t.scalar_type() == type && t.dim() == 1 && t.numel() == n && t.is_contiguous() &&
@@ -375,7 +813,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   auto tokens = at::empty({B, max_q}, ids.options());
   auto counts = at::empty({B}, cu_q.options());
   if (B == 0) return {tokens, counts, 0};
-  auto scratch = at::empty({R * 2}, ids.options());
+  auto scratch = at::empty({R * 2}, ids.options());  // cut, then largest logit and acceptance
   VerifyArgs a{};
   a.logits = logits.data_ptr();
   a.ld = logits.stride(0);
@@ -396,17 +834,31 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   a.tokens = tokens.data_ptr<int64_t>();
   a.counts = counts.data_ptr<int>();
   a.cut = reinterpret_cast<unsigned long long*>(scratch.data_ptr<int64_t>());
-  a.accept = reinterpret_cast<int*>(scratch.data_ptr<int64_t>() + R);
+  a.row_max = reinterpret_cast<float*>(scratch.data_ptr<int64_t>() + R);
+  a.accept = reinterpret_cast<int*>(a.row_max + R);
   a.err = err.data_ptr<int>();
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool wide = logits.scalar_type() == at::kFloat;
+  const int64_t width = wide ? 4 : 2;
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // CTAs per row: two of them fit an SM (their slices at most 80 KB), more while SMs would idle
+  auto cluster_for = [&](int64_t count) {
+    int64_t n = 1;
+    while (n < kMaxCluster && (V * width > n * 80 * 1024 || count * n * 2 <= sms)) n *= 2;
+    return n;
+  };
+  auto run = [&](auto kern, int64_t count) {
+    const int64_t n = cluster_for(count);
+    const size_t smem = (size_t)(((V + n - 1) / n + 7) / 8 * 8 * width + 32);
+    TORCH_CHECK(smem <= 190 * 1024, "the vocabulary does not fit the shared memory of a cluster");
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    C10_CUDA_CHECK(nvb::launch_cluster(kern, dim3((unsigned)(n * count)), dim3(kThreads), smem, stream, (unsigned)n, a));
+  };
   if (R > 0) {
-    C10_CUDA_CHECK(nvb::launch(wide ? verify_rows_kernel<float> : verify_rows_kernel<bf16>, dim3((unsigned)R),
-                               dim3(kThreads), 0, stream, a));
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    if (wide) run(verify_rows_kernel<float>, R);
+    else run(verify_rows_kernel<bf16>, R);
   }
-  C10_CUDA_CHECK(nvb::launch(wide ? verify_draw_kernel<float> : verify_draw_kernel<bf16>, dim3((unsigned)B),
-                             dim3(kThreads), 0, stream, a));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (wide) run(verify_draw_kernel<float>, B);
+  else run(verify_draw_kernel<bf16>, B);
   return {tokens, counts, R > 0 ? 2 : 1};
 }

@@ -567,7 +567,8 @@ def verify_drafts(logits, ids, cu_q, max_q, temps, top_ks, top_ps, uniforms, dra
     Draft d of row r is accepted while uniforms[r] * q[d] < p[d].  The token after the accepted drafts is drawn from
     max(0, p - q) of the refused row (without q: p without d), or from p of the last row when none was refused, by the
     inverse of its cumulated sum in token order with the uniform of the sequence's last row (fp32 or fp64, [0, 1)), so
-    the emitted tokens are distributed as tokens sampled one by one.  A draft outside the vocabulary is refused.
+    the emitted tokens are distributed as tokens sampled one by one.  A draft outside the vocabulary is refused; a token
+    whose logit is -inf or NaN is never drawn (a row without any other draws token 0).
 
     Returns (tokens int64 [B, max_q]: accepted drafts, the drawn token, then -1; counts int32 [B]: tokens emitted, 0
     for a sequence without rows).  A sequence of more than ``max_q`` rows is reported by ``check_device_errors`` and
@@ -576,7 +577,7 @@ def verify_drafts(logits, ids, cu_q, max_q, temps, top_ks, top_ps, uniforms, dra
         R, V = logits.shape
         B = cu_q.numel() - 1
         _require(logits.dtype in (torch.bfloat16, torch.float32), "logits must be bf16 or fp32 [rows, vocabulary]")
-        _require(1 <= V <= 1 << 20, "the vocabulary must have 1 to 1048576 tokens")
+        _require(1 <= V <= 327680, "the vocabulary must have 1 to 327680 tokens")
         for t, dtypes, n, name in ((cu_q, (torch.int32,), B + 1, "cu_q"), (ids, (torch.int64,), R, "ids"),
                                    (temps, (torch.float32,), B, "temps"), (top_ks, (torch.int32,), B, "top_ks"),
                                    (top_ps, (torch.float32,), B, "top_ps"),

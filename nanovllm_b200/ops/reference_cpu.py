@@ -353,7 +353,7 @@ def target_probs(logits: torch.Tensor, temp: float, top_k: int, top_p: float, so
     order = torch.sort(-raw, stable=True).indices  # value descending, index ascending on ties
     top = raw == m
     w = torch.where(top, torch.ones_like(x), torch.exp((x - x[order[0]]) / temp))
-    w = torch.where((raw == float("-inf")) & (softcap <= 0), torch.zeros_like(w), w)
+    w = torch.where(raw == float("-inf"), torch.zeros_like(w), w)  # masked stays masked, also under a soft-cap
     if top_k == 1:  # whatever the temperature is
         w = top.double()
     n = V if top_k <= 0 or top_k > V else top_k

@@ -20,7 +20,7 @@ def probs_of(row, temp, k, top, cap):
     if m == -math.inf:
         return [0.0] * len(x)
     capped = (lambda v: cap * math.tanh(v / cap)) if cap else (lambda v: v)
-    w = [1.0 if v == m else math.exp(max(-1e4, (capped(v) - capped(m)) / temp)) for v in x]
+    w = [1.0 if v == m else 0.0 if v == -math.inf else math.exp(max(-1e4, (capped(v) - capped(m)) / temp)) for v in x]
     kept = order if k <= 0 or k > len(x) else order[:k]
     if top < 1.0:
         total, mass, n = math.fsum(w[i] for i in kept), 0.0, 0
@@ -131,6 +131,34 @@ def test_mixed_requests_and_ties(dtype, dev):
 def test_softcap(k, top, dev):
     s = dict(make([3, 1, 5], 400, 7, 0.9, k, top, True, spread=12.0), softcap=10.0)
     assert call(s, dev) == tuple(oracle(s))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("k,top", [(0, 1.0), (5, 0.8)])
+def test_masks_under_a_softcap(k, top, dev):
+    s = dict(make([3, 1, 4], 300, 43, 0.9, k, top, True, spread=12.0), softcap=10.0)
+    s["logits"][:, ::2] = -math.inf
+    s["logits"][:, 5::4] = math.nan
+    s["logits"][2] = -math.inf
+    assert call(s, dev) == tuple(oracle(s))
+
+
+@gpu
+@pytest.mark.parametrize("V", [9001, 70000, 151936])
+@pytest.mark.parametrize("k,top", [(0, 0.95), (0, 0.5), (2000, 1.0), (3000, 0.9), (30, 0.9), (0, 1.0), (10 ** 5, 0.9)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_flat_and_steep_rows(V, k, top, dtype):
+    """Cuts among few tokens (sorted) and among many thousand (radix select), with many equal logits, against the CPU
+    restatement in 64 bits; rows with one far token, rows of few values, rows of one value."""
+    s = make([3, 3, 2, 4], V, V + k, 1.0, k, top, True, dtype, spread=1.0)
+    x = s["logits"]
+    x[1] = x[1] * 4
+    x[3, 17] = 40.0
+    x[4] = torch.round(x[4])
+    x[6] = 1.5
+    x[8, 100:] = -50.0
+    x[9] = torch.linspace(-9, 9, V).to(dtype)
+    assert call(s, "cuda") == call(s, "cpu")
 
 
 @pytest.mark.parametrize("dev", DEVICES)
