@@ -13,6 +13,7 @@
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cfloat>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -31,7 +32,7 @@ constexpr int kMaxVocab = 327680;  // 32-bit logits of a row in the shared memor
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 128;   // of 1/8 octave of weight below the row's largest; the last one holds the rest
 constexpr int kList = 1024;  // tokens that a cut is found among by sorting
-constexpr float kListMargin = 1.0001f;
+constexpr float kListMargin = 1.0001f;  // of sums of 32-bit weights
 
 struct VerifyArgs {
   const void* logits;
@@ -80,20 +81,22 @@ NV_DEVICE unsigned long long rank_key(float x, int i) {
   return ((unsigned long long)order_key(fmaxf(x, -INFINITY) + 0.f) << 32) | (0xffffffffu - (uint32_t)i);
 }
 
-// 2^y for y <= 0 in 64 bits (relative error below 1e-13): y = k / 64 + r, a table of 2^(k / 64) and a polynomial for
-// 2^r, |r| <= 1/128 (the remainder of the exponential series behind the fourth power is 4e-14).
-NV_DEVICE double exp2_neg(double y, const double* table) {
-  if (!(y > -1000.0)) return 0.0;
-  const double magic = 105553116266496.0;  // 1.5 * 2^46: the last bit of y + magic is 1/64
-  const double t = y + magic;
-  const double r = y - (t - magic);
-  const int k = __double2loint(t);
-  double p = 9.618129107628477e-3;
-  p = fma(p, r, 5.550410866482158e-2);
+// 2^(d c) in 64 bits (relative error below 1e-12) for an exponent in [-1000, 0]: it is k / 256 + r, with a table of
+// 2^(k / 256) and three terms of the exponential series for 2^r, |r| <= 1/512 (the fourth is 1.4e-13).
+constexpr int kTable = 256;
+NV_DEVICE double exp2_64(double d, double c, const double* table) {
+  const double magic = 26388279066624.0;  // 1.5 * 2^44: the last bit of a sum with it is 1/256
+  const double t = fma(d, c, magic);
+  const double r = fma(d, c, magic - t);
+  const int k = max(__double2loint(t), -1000 * kTable);
+  double p = 5.550410866482158e-2;
   p = fma(p, r, 2.402265069591007e-1);
   p = fma(p, r, 6.931471805599453e-1);
-  p = fma(p, r, 1.0) * table[k & 63];
-  return __hiloint2double(__double2hiint(p) + (k >> 6) * (1 << 20), __double2loint(p));
+  p = fma(p, r, 1.0) * table[k & (kTable - 1)];
+  return __hiloint2double(__double2hiint(p) + (k >> 8) * (1 << 20), __double2loint(p));
+}
+NV_DEVICE void fill_table(double* table) {
+  if (threadIdx.x < kTable) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / kTable));
 }
 
 // Weights of a row relative to its largest logit.  ``weight`` (32 bits) takes the exponent's argument as a product with
@@ -102,7 +105,8 @@ NV_DEVICE double exp2_neg(double y, const double* table) {
 struct RowScale {
   float m, softcap, mc;  // largest logit, its capped value
   float c_hi, c_lo;      // log2(e) / T
-  double m64, c64, cap64;
+  float floor64;         // logits below it weigh nothing in 64 bits (2^-1000)
+  double c64, m64, cap64;  // m64: the capped largest logit
 
   NV_DEVICE RowScale(float m_, float cap, float T) : m(m_), softcap(cap) {
     c64 = kLog2e64 / (double)T;
@@ -111,6 +115,7 @@ struct RowScale {
     cap64 = cap;
     mc = capped(m);
     m64 = capped64(m);
+    floor64 = fmaxf(softcap > 0.f ? -FLT_MAX : m - 690.f * T, -FLT_MAX);
   }
   NV_DEVICE float capped(float x) const {
     if (softcap <= 0.f) return x;
@@ -118,17 +123,29 @@ struct RowScale {
     return softcap * (1.f - 2.f / (e + 1.f));
   }
   NV_DEVICE double capped64(float x) const { return softcap > 0.f ? cap64 * tanh((double)x / cap64) : (double)x; }
+  NV_DEVICE bool simple() const { return softcap <= 0.f && fabsf(m) < INFINITY; }
   // log2 of the weight; hugely negative for NaN, -inf and the type's lowest value (no product to overflow)
+  NV_DEVICE float log_weight_simple(float x) const {
+    const float d = fmaxf(x - m, -1e30f);
+    return fmaf(d, c_hi, d * c_lo);
+  }
   NV_DEVICE float log_weight(float x) const {
     if (m == INFINITY) return x == m ? 0.f : -1e30f;
-    const float d = softcap > 0.f && x == -INFINITY ? -1e30f : fmaxf(capped(x) - mc, -1e30f);
+    if (softcap <= 0.f) return log_weight_simple(x);
+    const float d = x == -INFINITY ? -1e30f : fmaxf(capped(x) - mc, -1e30f);
     return fminf(0.f, fmaf(d, c_hi, d * c_lo));
   }
   NV_DEVICE float weight(float x) const { return exp2f(log_weight(x)); }
+  NV_DEVICE double weight64_simple(float x, const double* table) const {  // no soft-cap, finite m
+    const double w = exp2_64((double)fmaxf(x, floor64) - m64, c64, table);
+    return x >= floor64 ? w : 0.0;  // NaN, -inf: 0
+  }
   NV_DEVICE double weight64(float x, const double* table) const {
     if (x == m) return m == -INFINITY ? 0.0 : 1.0;
-    const double d = x == -INFINITY ? -1e300 : capped64(x) - m64;  // masked stays masked, also under a soft-cap
-    return d > -1e30 ? exp2_neg(fmin(0.0, d * c64), table) : 0.0;  // NaN: 0
+    if (m == INFINITY || !(x >= floor64)) return 0.0;  // masked stays masked, also under a soft-cap
+    if (softcap <= 0.f) return weight64_simple(x, table);
+    const double d = fmin(capped64(x) - m64, 0.0);
+    return d * c64 > -1000.0 ? exp2_64(d, c64, table) : 0.0;
   }
 };
 
@@ -222,6 +239,7 @@ struct Slice {
   static constexpr int PER = 16 / sizeof(T);
   const T* words;  // 16-byte aligned
   int lo, hi, nw, first;  // token of word w, element e: first + w * PER + e
+  bool bulk;
 
   template <typename F>
   NV_DEVICE void each(int w, F f) const {
@@ -234,8 +252,9 @@ struct Slice {
 
 NV_DEVICE int slice_tokens(int V, int n) { return ((V + n - 1) / n + 7) / 8 * 8; }
 
+// Starts the load; ``finish_slice`` before the words are read.
 template <typename T>
-NV_DEVICE Slice<T> load_slice(const T* row, int V, uint8_t* buf, uint64_t* bar, int* err) {
+NV_DEVICE Slice<T> load_slice(const T* row, int V, uint8_t* buf, uint64_t* bar) {
   Slice<T> s;
   const int per = slice_tokens(V, cluster_size()), tid = threadIdx.x;
   s.lo = min(V, (int)nvb::cluster_ctarank() * per);
@@ -268,13 +287,13 @@ NV_DEVICE Slice<T> load_slice(const T* row, int V, uint8_t* buf, uint64_t* bar, 
   if (tid < n_head) el[skip + tid] = row[s.lo + tid];
   if (tid < n_tail) el[skip + n - n_tail + tid] = row[s.hi - n_tail + tid];
   for (int i = skip + n + tid; i < s.nw * Slice<T>::PER; i += kThreads) el[i] = (T)(-INFINITY);
-  __syncthreads();
-  if (bulk) nvb::mbar_wait(bar, 0, err, nullptr);
+  s.bulk = bulk;
   return s;
 }
-
-NV_DEVICE void fill_table(double* table) {
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x / 64.0);
+template <typename T>
+NV_DEVICE void finish_slice(const Slice<T>& s, uint64_t* bar, int* err) {
+  __syncthreads();
+  if (s.bulk) nvb::mbar_wait(bar, 0, err, nullptr);
 }
 
 // One cluster per row: the kept set and, where the row holds a draft, its acceptance.  The row stays in the cluster's
@@ -291,11 +310,13 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
   extern __shared__ __align__(128) uint8_t buf[];
   __shared__ uint64_t bar;
   __shared__ float sh_f[32], slot_f;
-  __shared__ double sh_d[32], slot_d[3], table[64];
+  __shared__ double sh_d[32], slot_d[3], table[kTable];
   __shared__ int sh_i[32];
-  __shared__ unsigned long long sh_u[32], slot_u[2];
+  __shared__ unsigned long long sh_u[32], slot_u[4];
+  __shared__ float slot_f3[2][2];
   __shared__ unsigned int hist[kBins], hist_all[kBins];
   __shared__ unsigned long long hist_m[2][256];
+  __shared__ unsigned int hist_c[2][256];
   __shared__ unsigned long long keys[kList];
   __shared__ unsigned int n_list, slot_n;
   __shared__ int sel[4];
@@ -303,14 +324,15 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
   __shared__ double z_sh;
   const int r = blockIdx.x / cluster_size(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
+  const T* x = reinterpret_cast<const T*>(a.logits) + r * a.ld;
+  const Slice<T> s = load_slice(x, V, buf, &bar);
   const int b = seq_of_row(a.cu_q, a.B, r);
   const int2 rows = seq_rows(a, b);
-  if (r < rows.x || r >= rows.y) return;  // the whole cluster
   fill_table(table);
   if (tid < kBins) hist[tid] = 0;
   if (tid == 0) n_list = 0;
-  const T* x = reinterpret_cast<const T*>(a.logits) + r * a.ld;
-  const Slice<T> s = load_slice(x, V, buf, &bar, a.err);
+  finish_slice(s, &bar, a.err);
+  if (r < rows.x || r >= rows.y) return;  // the whole cluster
   float m = -INFINITY;
   for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { m = fmaxf(m, v); });
   m = cluster_max(m, sh_f, &slot_f);
@@ -342,16 +364,21 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
   } else {
     const bool cuts = (cut_k || cut_p) && m != -INFINITY;
     float z4[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int w = tid; w < s.nw; w += kThreads) {
-      int j = 0;
-      s.each(w, [&](float v, int) {
-        const float lw = rs.log_weight(v);
-        z4[j++ & 3] += exp2f(lw);
-        if (cuts) {
-          const int bin = (int)fminf(lw * -8.f, (float)(kBins - 1));
-          if (bin < kBins - 1) atomicAdd(&hist[bin], 1u);
-        }
-      });
+    if (!cuts && rs.simple()) {
+      for (int w = tid; w < s.nw; w += kThreads) {
+        int j = 0;
+        s.each(w, [&](float v, int) { z4[j++ & 3] += exp2f(rs.log_weight_simple(v)); });
+      }
+    } else {
+      const bool simple = rs.simple();
+      for (int w = tid; w < s.nw; w += kThreads) {
+        int j = 0;
+        s.each(w, [&](float v, int) {
+          const float lw = simple ? rs.log_weight_simple(v) : rs.log_weight(v);
+          z4[j++ & 3] += exp2f(lw);
+          if (cuts && lw > -(kBins - 1) / 8.f) atomicAdd(&hist[(int)(lw * -8.f)], 1u);
+        });
+      }
     }
     Z = cluster_sum((double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]), sh_d, &slot_d[0]);
     if (cuts) {
@@ -363,66 +390,64 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
       }
       __syncthreads();
       if (warp == 0) {
-        // lane: 4 bins.  lowest and highest mass that the counts allow, from the largest weights on
+        // lane: 4 bins.  Counts, and the lowest, middle and highest mass that they allow, from the largest weights on
         unsigned int cnt = 0;
-        float low = 0.f, high = 0.f;
+        float low = 0.f, mid = 0.f, high = 0.f;
         unsigned int c4[4];
-        float l4[4], h4[4];
+        float l4[4], m4[4], h4[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int bin = lane * 4 + j;
           const unsigned int n = bin < kBins - 1 ? hist_all[bin] : 0u;
           c4[j] = cnt += n;
           l4[j] = low += n * exp2f((bin + 1.01f) * -0.125f);
+          m4[j] = mid += n * exp2f((bin + 0.5f) * -0.125f);
           h4[j] = high += n * exp2f((bin - 0.01f) * -0.125f);
         }
         unsigned int ci = cnt;
-        float li = low, hi = high;
+        float li = low, mi = mid, hi = high;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const unsigned int cu = __shfl_up_sync(0xffffffffu, ci, o);
-          const float lu = __shfl_up_sync(0xffffffffu, li, o), hu = __shfl_up_sync(0xffffffffu, hi, o);
-          if (lane >= o) ci += cu, li += lu, hi += hu;
+          const float lu = __shfl_up_sync(0xffffffffu, li, o), mu = __shfl_up_sync(0xffffffffu, mi, o);
+          const float hu = __shfl_up_sync(0xffffffffu, hi, o);
+          if (lane >= o) ci += cu, li += lu, mi += mu, hi += hu;
         }
-        const float want = (float)((double)top * Z);
-        // first bin that certainly / possibly reaches the target
-        int sure_k = kBins - 1, sure_p = kBins - 1, may_p = kBins - 1;
+        const float want = (float)((double)top * Z), likely = 0.5f * (want + (float)Z);
+        // first bin that certainly / probably / possibly reaches the target, and the last one that the list holds
+        int sure_k = kBins - 1, sure_p = kBins - 1, prob_p = kBins - 2, may_p = kBins - 1, fit = -1;
 #pragma unroll
         for (int j = 3; j >= 0; --j) {
           const int bin = lane * 4 + j;
           if (bin >= kBins - 1) continue;
           if (ci - cnt + c4[j] >= (unsigned int)k) sure_k = bin;
           if (li - low + l4[j] >= want * kListMargin) sure_p = bin;
+          if (mi - mid + m4[j] >= likely) prob_p = bin;
           if (hi - high + h4[j] >= want / kListMargin) may_p = bin;
+          if (ci - cnt + c4[j] <= (unsigned int)kList) fit = max(fit, bin);
         }
         sure_k = __reduce_min_sync(0xffffffffu, sure_k);
         sure_p = __reduce_min_sync(0xffffffffu, sure_p);
+        prob_p = __reduce_min_sync(0xffffffffu, prob_p);
         may_p = __reduce_min_sync(0xffffffffu, may_p);
+        fit = __reduce_max_sync(0xffffffffu, fit);
         if (lane == 0) {
           sel[0] = sure_k;
           sel[1] = sure_p;
           sel[2] = may_p;
+          // one bin more than the one that holds the cut; a list that turns out short of the mass is given up again
+          sel[3] = cut_k ? (sure_k + 1 <= fit ? sure_k + 1 : -1) : min(prob_p + 1, fit);
         }
-        // tokens up to the bin after the one that certainly holds the cut
-        const int need = min(kBins - 1, (cut_k ? sure_k : sure_p) + 1);
-        unsigned int at = need < kBins - 1 && (cut_k ? sure_k : sure_p) < kBins - 1 ? 0u : 0xffffffffu;
-        if (at == 0u) {
-          const unsigned int upto = __shfl_sync(0xffffffffu, ci - cnt, need / 4);
-          unsigned int in4 = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j == need % 4) in4 = c4[j];
-          at = upto + __shfl_sync(0xffffffffu, in4, need / 4);
-        }
-        if (lane == 0) sel[3] = at <= (unsigned int)kList ? need : -1;
       }
       __syncthreads();
       const int last_bin = sel[3];
-      if (last_bin >= 0) {
+      bool listed = last_bin >= 0;
+      if (listed) {
         // ------------------------------------------------ few tokens: collect, sort, walk
         for (int w = tid; w < s.nw; w += kThreads)
           s.each(w, [&](float v, int i) {
-            if ((int)fminf(rs.log_weight(v) * -8.f, (float)(kBins - 1)) <= last_bin)
+            const float lw = rs.log_weight(v);
+            if (lw > -(kBins - 1) / 8.f && (int)(lw * -8.f) <= last_bin)
               keys[atomicAdd(&n_list, 1u)] = rank_key(v, i);
           });
         __syncthreads();
@@ -484,6 +509,7 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
             all += sh_d[i];
           }
           const double want = cut_p ? (double)top * (cut_k ? all : Z) : 4.0 * kMaxVocab;
+          listed = cut_k || all >= want;  // with a token of each bin behind the cut's, roundings of the weights included
           double before = base + incl - sum, kept = 0.0;
           int last = -1;
 #pragma unroll
@@ -504,35 +530,88 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
             z_sh = kept;
           }
           __syncthreads();
-          cut = cut_sh;
-          Z = z_sh;
+          if (listed) {
+            cut = cut_sh;
+            Z = z_sh;
+          }
+          if (tid == 0) sel_u[0] = listed;
+          __syncthreads();
         }
-      } else {
-        // ------------------------------------------------ many: radix select, 8 bits a pass, over the tokens of bins
-        // [from, upto]; all tokens of the bins before are kept
-        auto bin_of = [&](float v) { return (int)fminf(rs.log_weight(v) * -8.f, (float)(kBins - 1)); };
+        if (CL > 1 && !cut_k) {
+          nvb::cluster_sync();
+          listed = peer_load(&sel_u[0], 0) != 0;
+          nvb::cluster_sync();
+        }
+      }
+      if (!listed) {
+        // ------------------------------------------------ many: radix select over the tokens whose logits lie in the
+        // range of those in the bins in question
+        auto bin_of = [&](float v) {
+          const float lw = rs.log_weight(v);
+          return lw > -(kBins - 1) / 8.f ? (int)(lw * -8.f) : kBins - 1;
+        };
+        // sum of 1 or of the masses over f(logit, token)
+        auto total_of = [&](bool by_mass, unsigned long long* slot, auto f) {
+          unsigned long long n = 0;
+          for (int w = tid; w < s.nw; w += kThreads)
+            s.each(w, [&](float v, int i) {
+              if (i >= s.lo && i < s.hi && f(v, i)) n += by_mass ? (unsigned long long)(rs.weight(v) * kUnit) : 1ull;
+            });
+          return cluster_sum(n, sh_u, slot);
+        };
         int flip = 0;
-        auto select = [&](bool by_mass, unsigned long long target, unsigned long long before, int from, int upto,
-                          unsigned long long floor_key) {
-          unsigned long long prefix = 0, mask = 0;
-          for (int shift = 56; shift >= 0; shift -= 8) {
+        // the smallest kept key when 1 or masses are summed in descending key order up to ``target``, of the keys >= floor
+        auto select = [&](bool by_mass, unsigned long long target, int from, int upto, unsigned long long floor_key,
+                          int slot) {
+          float lo = -INFINITY, hi = -INFINITY;  // -smallest and largest logit
+          for (int w = tid; w < s.nw; w += kThreads)
+            s.each(w, [&](float v, int i) {
+              const int bin = bin_of(v);
+              if (bin < from || bin > upto || i < s.lo || i >= s.hi) return;
+              v = fmaxf(v, -INFINITY);
+              lo = fmaxf(lo, -v);
+              hi = fmaxf(hi, v);
+            });
+          lo = -cluster_max(lo, sh_f, &slot_f3[slot][0]);
+          hi = cluster_max(hi, sh_f, &slot_f3[slot][1]);
+          unsigned long long before = total_of(by_mass, &slot_u[slot * 2 + 1], [&](float v, int i) {
+            return v > hi && rank_key(v, i) >= floor_key;
+          });
+          // bits that differ: of the logits, then of the tokens
+          const uint32_t diff = order_key(lo + 0.f) ^ order_key(hi + 0.f);
+          const int token_bits = 32 - __clz(V - 1);
+          int bits = diff != 0 ? 64 - __clz(diff) : token_bits;
+          const unsigned long long top_key = (unsigned long long)order_key(hi + 0.f) << 32 | 0xffffffffull;
+          unsigned long long prefix = bits < 64 ? top_key >> bits << bits : 0ull;
+          while (bits > 0) {
+            const int nb = min(8, bits > 32 ? bits - 32 : bits), shift = bits - nb;
+            const unsigned int bin_mask = (1u << nb) - 1;
             unsigned long long* h = hist_m[flip];
-            for (int i = tid; i < 256; i += kThreads) h[i] = 0;
+            unsigned int* hc = hist_c[flip];
+            if (tid < 256) h[tid] = 0, hc[tid] = 0;
             __syncthreads();
             for (int w = tid; w < s.nw; w += kThreads)
               s.each(w, [&](float v, int i) {
-                const int bin = bin_of(v);
+                if (!(v <= hi) && !isnan(v)) return;
+                if (v < lo || i < s.lo || i >= s.hi) return;
                 const unsigned long long key = rank_key(v, i);
-                if (bin >= from && bin <= upto && key >= floor_key && (key & mask) == prefix && i >= s.lo && i < s.hi)
-                  atomicAdd(&h[(key >> shift) & 255], by_mass ? (unsigned long long)(rs.weight(v) * kUnit) : 1ull);
+                if (key < floor_key || (bits < 64 ? (key ^ prefix) >> bits : 0ull) != 0) return;
+                const unsigned int bin = (unsigned int)(key >> shift) & bin_mask;
+                atomicAdd(&hc[bin], 1u);
+                if (by_mass) atomicAdd(&h[bin], (unsigned long long)(rs.weight(v) * kUnit));
               });
             __syncthreads();
             if (CL > 1) nvb::cluster_sync();
             // every CTA adds up the cluster's bins and finds the same one
             if (tid < 256) {
               unsigned long long v = 0;
-              for (uint32_t i = 0; i < CL; ++i) v += CL > 1 ? peer_load(&h[tid], i) : h[tid];
-              keys[tid] = v;
+              unsigned int c = 0;
+              for (uint32_t i = 0; i < CL; ++i) {
+                c += CL > 1 ? peer_load(&hc[tid], i) : hc[tid];
+                if (by_mass) v += CL > 1 ? peer_load(&h[tid], i) : h[tid];
+              }
+              keys[tid] = by_mass ? v : c;
+              keys[256 + tid] = c;
             }
             __syncthreads();
             if (warp == 0) {  // lane: 8 bins from the top
@@ -550,43 +629,36 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
                 unsigned long long cum = before + incl - own;
                 int bin = 255 - lane * 8;
                 for (; bin > 248 - lane * 8 && cum + keys[bin] < target; --bin) cum += keys[bin];
-                sel_u[0] = prefix | ((unsigned long long)bin << shift);
+                sel_u[0] = prefix & ~(((unsigned long long)bin_mask) << shift) | ((unsigned long long)bin << shift);
                 sel_u[1] = cum;
+                sel[1] = keys[256 + bin] <= 1;
               }
             }
             __syncthreads();
-            prefix = sel_u[0];
+            prefix = sel_u[0] >> shift << shift;
             before = sel_u[1];
-            mask |= 255ull << shift;
+            const bool alone = sel[1] != 0;
+            bits = shift;
+            if (bits == 32 && token_bits < 32) {  // token bits above the vocabulary's are ones
+              bits = token_bits;
+              prefix |= 0xffffffffull >> token_bits << token_bits;
+            }
             flip ^= 1;  // the peers may still read the other one
             __syncthreads();
+            if (alone) break;  // no other key begins like this
           }
           return prefix;
         };
-        auto count_before = [&](int from) {
-          unsigned long long n = 0;
-          for (int i = 0; i < from; ++i) n += hist_all[i];
-          return n;
-        };
-        auto mass_of = [&](int upto, unsigned long long floor_key, unsigned long long* slot) {
-          unsigned long long z = 0;
-          for (int w = tid; w < s.nw; w += kThreads)
-            s.each(w, [&](float v, int i) {
-              if (bin_of(v) <= upto && rank_key(v, i) >= floor_key) z += (unsigned long long)(rs.weight(v) * kUnit);
-            });
-          return cluster_sum(z, sh_u, slot);
-        };
-        if (cut_k) {
-          const int from = max(0, sel[0] - 1);
-          cut = select(false, (unsigned long long)k, count_before(from), from, min(kBins - 1, sel[0] + 1), 0);
-        }
+        const int sure_k = sel[0], sure_p = sel[1], may_p = sel[2];
+        __syncthreads();
+        if (cut_k) cut = select(false, (unsigned long long)k, max(0, sure_k - 1), min(kBins - 1, sure_k + 1), 0, 0);
         if (cut_p) {
-          unsigned long long total = mass_of(kBins, cut, &slot_u[0]);
+          const unsigned long long total =
+              total_of(true, &slot_u[0], [&](float v, int i) { return rank_key(v, i) >= cut; });
           const double want = (double)total * (double)top;
           const unsigned long long target = want > 1.0 ? (unsigned long long)ceil(want) : 1ull;  // the first always stays
-          const int from = cut_k ? 0 : max(0, sel[2] - 1), upto = cut_k ? kBins - 1 : min(kBins - 1, sel[1] + 1);
-          const unsigned long long before = from > 0 ? mass_of(from - 1, cut, &slot_u[1]) : 0ull;
-          cut = max(cut, select(true, target, before, from, upto, cut));
+          cut = max(cut, select(true, target, cut_k ? 0 : max(0, may_p - 1), cut_k ? kBins - 1 : min(kBins - 1, sure_p + 1),
+                                cut, 1));
         }
         double z = 0.0;
         for (int w = tid; w < s.nw; w += kThreads) {
@@ -651,7 +723,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
   nvb::pdl_trigger();
   extern __shared__ __align__(128) uint8_t buf[];
   __shared__ uint64_t bar;
-  __shared__ double sh_d[32], slot_d, table[64], warp_sum_sh[2][kWarps], all_sh[kMaxCluster * kWarps + 1];
+  __shared__ double sh_d[32], slot_d, table[kTable], warp_sum_sh[2][kWarps], all_sh[kMaxCluster * kWarps + 1];
   __shared__ int sh_i[32];
   const int b = blockIdx.x / cluster_size(), tid = threadIdx.x, V = a.V, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
@@ -668,7 +740,6 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
     }
     return;
   }
-  fill_table(table);
   int acc = n - 1;  // accepted drafts: up to the first refusal
   for (int j0 = 0; j0 < n - 1; j0 += 32) {
     const bool no = j0 + lane < n - 1 && !a.accept[rows.x + j0 + lane];
@@ -680,32 +751,78 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
   }
   const int r = rows.x + acc;
   const bool rejected = acc < n - 1;
-  const Slice<T> s = load_slice(reinterpret_cast<const T*>(a.logits) + r * a.ld, V, buf, &bar, a.err);
+  const Slice<T> s = load_slice(reinterpret_cast<const T*>(a.logits) + r * a.ld, V, buf, &bar);
   const unsigned long long cut = a.cut[r];
   const RowScale rs(a.row_max[r], a.softcap, a.temps[b]);
   const int dr = rejected && a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
   const float* q = rejected && a.probs != nullptr && dr < a.D ? a.probs + dr * a.probs_ld : nullptr;
   const long drafted = rejected && a.probs == nullptr ? a.ids[r + 1] : -1;
-  auto weight = [&](float v, int i) { return rank_key(v, i) >= cut && i >= s.lo && i < s.hi ? rs.weight64(v, table) : 0.0; };
+  fill_table(table);
+  finish_slice(s, &bar, a.err);
+  const bool simple = cut == 0 && rs.simple();
+  const float cut_logit = cut == 0 ? -INFINITY : key_logit(cut);
+  constexpr int PER = Slice<T>::PER;
+  // weights of a word's tokens (what a slice's first and last word hold besides weighs nothing)
+  auto word_weights = [&](int w, double (&l)[PER]) {
+    const uint4 raw = reinterpret_cast<const uint4*>(s.words)[w];
+    const T* e = reinterpret_cast<const T*>(&raw);
+    if (simple) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) l[j] = rs.weight64_simple(to_float(e[j]), table);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const float v = to_float(e[j]);  // with a cut most tokens are below its logit
+        l[j] = v >= cut_logit && rank_key(v, s.first + w * PER + j) >= cut ? rs.weight64(v, table) : 0.0;
+      }
+    }
+  };
   double Zinv = 1.0;
   if (q != nullptr) {  // p - q needs p itself
-    double z = 0.0;
-    for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int i) { z += weight(v, i); });
+    double z = 0.0, l[PER];
+    for (int w = tid; w < s.nw; w += kThreads) {
+      word_weights(w, l);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) z += l[j];
+    }
     const double Z = cluster_sum(z, sh_d, &slot_d);
     Zinv = Z > 0.0 ? 1.0 / Z : 0.0;
   }
+  const bool q_aligned = q != nullptr && ((reinterpret_cast<uintptr_t>(q) + 4 * (long)s.first) & 15) == 0;
+  // what is left of a word's tokens to draw from; plain: the probabilities themselves
+  auto word_left = [&](int w, bool plain, double (&l)[PER]) {
+    word_weights(w, l);
+    if (plain) return;
+    const int i0 = s.first + w * PER;
+    if (q == nullptr) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) l[j] = i0 + j == drafted ? 0.0 : l[j];
+    } else {
+      float qv[PER];
+      if (q_aligned && i0 >= s.lo && i0 + PER <= s.hi) {
+#pragma unroll
+        for (int j = 0; j < PER; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(q + i0 + j);
+          qv[j] = v.x, qv[j + 1] = v.y, qv[j + 2] = v.z, qv[j + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) qv[j] = i0 + j >= s.lo && i0 + j < s.hi ? q[i0 + j] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < PER; ++j) l[j] = l[j] > 0.0 ? fmax(0.0, l[j] * Zinv - (double)qv[j]) : 0.0;
+    }
+  };
   // warps own consecutive words, lanes one word at a time
   const int per = (s.nw + kWarps - 1) / kWarps, w0 = min(s.nw, warp * per), w1 = min(s.nw, w0 + per);
   for (int plain = rejected ? 0 : 1; plain < 2; ++plain) {
-    // plain: the probabilities themselves (also when nothing is left of p - q)
-    auto left = [&](float v, int i) {
-      const double w = weight(v, i);
-      if (plain || w == 0.0) return w;
-      if (q != nullptr) return fmax(0.0, w * Zinv - (double)q[i]);
-      return i == drafted ? 0.0 : w;
-    };
-    double sum = 0.0;
-    for (int w = w0 + lane; w < w1; w += 32) s.each(w, [&](float v, int i) { sum += left(v, i); });
+    // plain: the probabilities themselves, also when nothing is left of p - q
+    double sum = 0.0, l[PER];
+    for (int w = w0 + lane; w < w1; w += 32) {
+      word_left(w, plain != 0, l);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) sum += l[j];
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) warp_sum_sh[plain][warp] = sum;
@@ -740,7 +857,11 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
         int tok = -1;
         for (int wb = w0; wb < w1; wb += 32) {
           double mine = 0.0;
-          if (wb + lane < w1) s.each(wb + lane, [&](float v, int i) { mine += left(v, i); });
+          if (wb + lane < w1) {
+            word_left(wb + lane, plain != 0, l);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) mine += l[j];
+          }
           double incl = mine;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -753,11 +874,11 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
           int cand = -1;
           if (lane == src) {
             double d = c + incl - mine;
-            s.each(wb + lane, [&](float v, int i) {
-              const double l = left(v, i);
-              if (l > 0.0 && !(cand >= 0 && d > want)) cand = i;
-              d += l;
-            });
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+              if (l[j] > 0.0 && !(cand >= 0 && d > want)) cand = s.first + (wb + lane) * PER + j;
+              d += l[j];
+            }
           }
           if (src >= 0) tok = __shfl_sync(0xffffffffu, cand, src);
           if (over != 0) break;
