@@ -24,15 +24,16 @@
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr double kLog2e64 = 1.4426950408889634074;
-// masses in the radix select are integers (any order, same sum): 2^43 per unit, fewer than 2^20 weights of at most 1
-constexpr float kUnit = 8796093022208.0f;
 constexpr int kMaxVocab = 327680;  // 32-bit logits of a row in the shared memory of eight CTAs
 constexpr int kMaxCluster = 8;
-constexpr int kBins = 128;   // of 1/8 octave of weight below the row's largest; the last one holds the rest
-constexpr int kList = 1024;  // tokens that a cut is found among by sorting
-constexpr float kListMargin = 1.0001f;  // of sums of 32-bit weights
+constexpr int kBins = 256;   // of 1/16 octave of weight below the row's largest; the last one holds the rest
+constexpr float kPerOctave = 16.f;
+constexpr int kList = 256;     // tokens that a cut is found among by ranking
+constexpr int kOwnList = 128;  // of one CTA
+constexpr int kTop = 64;     // largest top_k that the list is tried for
+constexpr float kSlack = 1.0001f;  // of sums of 32-bit weights
 
 struct VerifyArgs {
   const void* logits;
@@ -169,40 +170,54 @@ NV_DEVICE T peer_load(const T* p, uint32_t rank) {  // the same variable of anot
 }
 
 template <typename T>
-NV_DEVICE T block_sum(T v, T* sh) {
+NV_DEVICE void peer_store(T* p, uint32_t rank, T v) {
+  const uint32_t at = nvb::map_peer(nvb::smem_u32(p), rank);
+  if constexpr (sizeof(T) == 8)
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(*reinterpret_cast<unsigned long long*>(&v)) : "memory");
+  else
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(*reinterpret_cast<uint32_t*>(&v)) : "memory");
+}
+
+// Reductions over the cluster with one barrier: every warp writes its values into every CTA's table, each thread then
+// reads its own CTA's, in the same order everywhere.  Two tables in turn: whoever writes one again has passed a barrier
+// that everybody reached after reading it.
+template <int N, bool MAX, typename T>
+NV_DEVICE void cluster_reduce(T (&v)[N], double (&tables)[2][3][kMaxCluster * kWarps], int& turn) {
+  constexpr int STRIDE = kMaxCluster * kWarps;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t n = cluster_size(), rank = nvb::cluster_ctarank();
+  T* t = reinterpret_cast<T*>(tables[turn & 1]);
+  ++turn;
+  auto join = [](T a, T b) { return MAX ? (a > b ? a : b) : a + b; };
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int k = 0; k < N; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[k] = join(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
+    if ((uint32_t)lane < n) peer_store(&t[k * STRIDE + rank * kWarps + warp], lane, v[k]);
+  }
+  nvb::cluster_sync();
+  const int entries = (int)n * kWarps;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    T x = lane < entries ? t[k * STRIDE + lane] : (MAX ? v[k] : (T)0);
+    if (lane + 32 < entries) x = join(x, t[k * STRIDE + lane + 32]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = join(x, __shfl_xor_sync(0xffffffffu, x, o));
+    v[k] = x;
+  }
+}
+// The cluster's CTAs are there once each has arrived: waited for before the first access to another's shared memory.
+NV_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+NV_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
+NV_DEVICE int block_sum(int v, int* sh) {
+  v = __reduce_add_sync(0xffffffffu, v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
-  T r = sh[0];
-  for (int i = 1; i < kWarps; ++i) r += sh[i];
+  int r = 0;
+  for (int i = 0; i < kWarps; ++i) r += sh[i];
   return r;
-}
-// Sum over the cluster, the same in every thread.  ``slot``: one for each call of a kernel.
-template <typename T>
-NV_DEVICE T cluster_sum(T v, T* sh, T* slot) {
-  v = block_sum(v, sh);
-  const uint32_t n = cluster_size();
-  if (n == 1) return v;
-  if (threadIdx.x == 0) *slot = v;
-  nvb::cluster_sync();
-  T r = peer_load(slot, 0);
-  for (uint32_t i = 1; i < n; ++i) r += peer_load(slot, i);
-  return r;
-}
-NV_DEVICE float cluster_max(float v, float* sh, float* slot) {
-  v = nvb::warp_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  for (int i = 0; i < kWarps; ++i) v = fmaxf(v, sh[i]);
-  const uint32_t n = cluster_size();
-  if (n == 1) return v;
-  if (threadIdx.x == 0) *slot = v;
-  nvb::cluster_sync();
-  for (uint32_t i = 0; i < n; ++i) v = fmaxf(v, peer_load(slot, i));
-  return v;
 }
 
 // Sequence of row r by a 32-way search of the warp: the last b with cu_q[b] <= r.
@@ -298,202 +313,238 @@ NV_DEVICE void finish_slice(const Slice<T>& s, uint64_t* bar, int* err) {
 
 // One cluster per row: the kept set and, where the row holds a draft, its acceptance.  The row stays in the cluster's
 // shared memory, every pass after the load reads it there; bound by the bytes of the logits.
-//   no cut     maximum, sum of the weights
+//   no cut     each CTA's maximum and sum of weights against it, joined by one exchange
 //   top_k 1    maximum, its lowest token
-//   cuts       counts by 1/8 octave of weight bound where the cut falls; the tokens above that (and one bin more, so
-//              that roundings of the weight do not matter) are sorted when they are few, else the tokens of the bins in
-//              question go through a radix select over composite keys
+//   cuts       some hundred of the largest logits are ranked and walked, in one CTA; a cut that lies beyond them (a flat
+//              row, a large top_k) is found by passes that sum what lies above three thresholds each
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyArgs a) {
   nvb::pdl_wait();
   nvb::pdl_trigger();
   extern __shared__ __align__(128) uint8_t buf[];
   __shared__ uint64_t bar;
-  __shared__ float sh_f[32], slot_f;
-  __shared__ double sh_d[32], slot_d[3], table[kTable];
-  __shared__ int sh_i[32];
-  __shared__ unsigned long long sh_u[32], slot_u[4];
-  __shared__ float slot_f3[2][2];
-  __shared__ unsigned int hist[kBins], hist_all[kBins];
-  __shared__ unsigned long long hist_m[2][256];
-  __shared__ unsigned int hist_c[2][256];
-  __shared__ unsigned long long keys[kList];
-  __shared__ unsigned int n_list, slot_n;
-  __shared__ int sel[4];
-  __shared__ unsigned long long sel_u[2], cut_sh;
-  __shared__ double z_sh;
+  __shared__ double red[2][3][kMaxCluster * kWarps], table[kTable], sh_d[kWarps];
+  __shared__ float sh_f[kWarps], threshold_sh;
+  __shared__ int sh_i[kWarps], sel[3];
+  __shared__ unsigned int hist[kBins], n_list, n_gather, n_range[2], eq_sh[2][kMaxCluster * kWarps];
+  __shared__ unsigned long long keys[kOwnList], found_sh[2];
+  // the threads' maxima, then rank 0's list (keys, and weights in order), then the row's bins, then the logits in question
+  __shared__ __align__(16) double pool[2 * kList];
+  float* maxima = reinterpret_cast<float*>(pool);
+  unsigned int* hist_all = reinterpret_cast<unsigned int*>(pool);
   const int r = blockIdx.x / cluster_size(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
+  cluster_arrive();
+  int turn = 0;
+  auto sum1 = [&](double v) {
+    double x[1] = {v};
+    cluster_reduce<1, false>(x, red, turn);
+    return x[0];
+  };
   const T* x = reinterpret_cast<const T*>(a.logits) + r * a.ld;
   const Slice<T> s = load_slice(x, V, buf, &bar);
   const int b = seq_of_row(a.cu_q, a.B, r);
   const int2 rows = seq_rows(a, b);
-  fill_table(table);
-  if (tid < kBins) hist[tid] = 0;
-  if (tid == 0) n_list = 0;
-  finish_slice(s, &bar, a.err);
-  if (r < rows.x || r >= rows.y) return;  // the whole cluster
-  float m = -INFINITY;
-  for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { m = fmaxf(m, v); });
-  m = cluster_max(m, sh_f, &slot_f);
-  const RowScale rs(m, a.softcap, a.temps[b]);
+  const bool in_seq = r >= rows.x && r < rows.y;
   const int k = a.topk[b];
-  const float top = a.topp[b];
+  const float top = a.topp[b], temp = a.temps[b];
+  // the draft's logit, probability and uniform come while the row does
+  const bool drafted = in_seq && r + 1 < rows.y;
+  long d = -1;
+  float d_logit = 0.f;
+  double uq = 0.0;
+  if (drafted && rank == 0) {
+    const int dr = a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
+    d = a.ids[r + 1];
+    if (a.probs != nullptr && dr >= a.D) {
+      if (tid == 0) nvb::record_error(a.err, nvb::kErrBadArgument);
+      d = -1;
+    }
+    if (d >= V) d = -1;
+    if (d >= 0) {
+      d_logit = to_float(x[d]);
+      uq = a.uniform(r) * (a.probs != nullptr ? (double)a.probs[dr * a.probs_ld + d] : 1.0);
+    }
+  }
+  fill_table(table);
+  for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
+  if (tid == 0) {
+    n_list = n_gather = n_range[0] = n_range[1] = 0;
+    found_sh[0] = found_sh[1] = 0;
+  }
+  finish_slice(s, &bar, a.err);
+  cluster_wait();
+  if (!in_seq) return;  // the whole cluster
+  float mine_max = -INFINITY;
+  for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { mine_max = fmaxf(mine_max, v); });
   const bool cut_k = k > 0 && k < V, cut_p = top < 1.f;
   unsigned long long cut = 0;
   double Z = 0.0;
+  float m;
+  if (!cut_k && !cut_p && a.softcap <= 0.f) {
+    // ---------------------------------------------------------------- no cut: sums against the CTA's own maximum
+    const float mw = nvb::warp_max(mine_max);
+    if (lane == 0) sh_f[warp] = mw;
+    __syncthreads();
+    float mc = sh_f[0];
+    for (int i = 1; i < kWarps; ++i) mc = fmaxf(mc, sh_f[i]);
+    const RowScale own(mc, 0.f, temp);
+    float z4[4] = {0.f, 0.f, 0.f, 0.f};
+    if (own.simple()) {
+      for (int w = tid; w < s.nw; w += kThreads) {
+        int j = 0;
+        s.each(w, [&](float v, int) { z4[j++ & 3] += exp2f(own.log_weight_simple(v)); });
+      }
+    } else if (mc == INFINITY) {
+      for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { z4[0] += v == INFINITY ? 1.f : 0.f; });
+    }
+    // warps' sums and the CTA's maximum to every CTA
+    double z = (double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if ((uint32_t)lane < CL) {
+      peer_store(&red[0][0][rank * kWarps + warp], lane, z);
+      peer_store(&red[0][1][rank * kWarps + warp], lane, (double)mc);
+    }
+    turn = 1;
+    nvb::cluster_sync();
+    float mx = -INFINITY;
+    for (int i = lane; i < (int)CL * kWarps; i += 32) mx = fmaxf(mx, (float)red[0][1][i]);
+    m = nvb::warp_max(mx);
+    const RowScale rs(m, 0.f, temp);
+    double t = 0.0;
+    for (int i = lane; i < (int)CL * kWarps; i += 32) {
+      const double zi = red[0][0][i];
+      if (zi > 0.0) t += zi * rs.weight64((float)red[0][1][i], table);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    Z = t;
+  } else {
+    float mv[1] = {mine_max};
+    cluster_reduce<1, true>(mv, red, turn);
+    m = mv[0];
+  }
+  const RowScale rs(m, a.softcap, temp);
+  const bool simple = rs.simple();
   if (k == 1) {
-    // the lowest token among the largest logits
-    unsigned long long best = 0;
+    // ---------------------------------------------------------------- greedy: the lowest token among the largest logits
+    unsigned long long best[1] = {0};
     for (int w = tid; w < s.nw; w += kThreads)
       s.each(w, [&](float v, int i) {
-        if (v == m) best = max(best, rank_key(v, i));
+        if (v == m && i >= s.lo && i < s.hi) best[0] = max(best[0], rank_key(v, i));
       });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane == 0) sh_u[warp] = best;
-    __syncthreads();
-    for (int i = 0; i < kWarps; ++i) best = max(best, sh_u[i]);
-    if (CL > 1) {
-      if (tid == 0) slot_u[0] = best;
-      nvb::cluster_sync();
-      for (uint32_t i = 0; i < CL; ++i) best = max(best, peer_load(&slot_u[0], i));
-    }
-    cut = m == -INFINITY ? 0 : best;
+    cluster_reduce<1, true>(best, red, turn);
+    cut = m == -INFINITY ? 0 : best[0];
     Z = 1.0;
-  } else {
+  } else if (cut_k || cut_p || a.softcap > 0.f) {
     const bool cuts = (cut_k || cut_p) && m != -INFINITY;
+    // With a cut: this CTA's tokens at or above its threshold, the want_top-th largest of its threads' maxima, so at least
+    // that many; the row's list holds every token at or above the largest threshold of the cluster.  A top_k needs
+    // top_k of them in case one CTA has them all, a top_p some 256 in the cluster.
+    const int want_top = cut_k ? min(k, kTop) : max(32, min(128, 256 / (int)CL));
+    if (cuts) {
+      maxima[tid] = mine_max;
+      __syncthreads();
+      if (warp == 0) {
+        uint32_t own[kThreads / 32], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+        for (int j = 0; j < kThreads / 32; ++j) {
+          own[j] = order_key(maxima[j * 32 + lane] + 0.f);
+          lo = min(lo, own[j]);
+          hi = max(hi, own[j]);
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        while (lo < hi) {  // at least want_top threads at lo
+          const uint32_t mid = lo + (hi - lo) / 2 + 1;
+          int n = 0;
+#pragma unroll
+          for (int j = 0; j < kThreads / 32; ++j) n += own[j] >= mid;
+          if (__reduce_add_sync(0xffffffffu, n) >= want_top) lo = mid;
+          else hi = mid - 1;
+        }
+        if (lane == 0) threshold_sh = key_logit((unsigned long long)lo << 32);
+      }
+    }
     float z4[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!cuts && rs.simple()) {
+    if (simple) {
       for (int w = tid; w < s.nw; w += kThreads) {
         int j = 0;
         s.each(w, [&](float v, int) { z4[j++ & 3] += exp2f(rs.log_weight_simple(v)); });
       }
     } else {
-      const bool simple = rs.simple();
       for (int w = tid; w < s.nw; w += kThreads) {
         int j = 0;
-        s.each(w, [&](float v, int) {
-          const float lw = simple ? rs.log_weight_simple(v) : rs.log_weight(v);
-          z4[j++ & 3] += exp2f(lw);
-          if (cuts && lw > -(kBins - 1) / 8.f) atomicAdd(&hist[(int)(lw * -8.f)], 1u);
-        });
+        s.each(w, [&](float v, int) { z4[j++ & 3] += rs.weight(v); });
       }
     }
-    Z = cluster_sum((double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]), sh_d, &slot_d[0]);
+    float threshold = -INFINITY;
     if (cuts) {
-      // counts of the whole row (the sum above was a barrier of the cluster, or of the only CTA)
-      if (tid < kBins - 1) {
-        unsigned int n = 0;
-        for (uint32_t i = 0; i < CL; ++i) n += CL > 1 ? peer_load(&hist[tid], i) : hist[tid];
-        hist_all[tid] = n;
-      }
       __syncthreads();
-      if (warp == 0) {
-        // lane: 4 bins.  Counts, and the lowest, middle and highest mass that they allow, from the largest weights on
-        unsigned int cnt = 0;
-        float low = 0.f, mid = 0.f, high = 0.f;
-        unsigned int c4[4];
-        float l4[4], m4[4], h4[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int bin = lane * 4 + j;
-          const unsigned int n = bin < kBins - 1 ? hist_all[bin] : 0u;
-          c4[j] = cnt += n;
-          l4[j] = low += n * exp2f((bin + 1.01f) * -0.125f);
-          m4[j] = mid += n * exp2f((bin + 0.5f) * -0.125f);
-          h4[j] = high += n * exp2f((bin - 0.01f) * -0.125f);
-        }
-        unsigned int ci = cnt;
-        float li = low, mi = mid, hi = high;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned int cu = __shfl_up_sync(0xffffffffu, ci, o);
-          const float lu = __shfl_up_sync(0xffffffffu, li, o), mu = __shfl_up_sync(0xffffffffu, mi, o);
-          const float hu = __shfl_up_sync(0xffffffffu, hi, o);
-          if (lane >= o) ci += cu, li += lu, mi += mu, hi += hu;
-        }
-        const float want = (float)((double)top * Z), likely = 0.5f * (want + (float)Z);
-        // first bin that certainly / probably / possibly reaches the target, and the last one that the list holds
-        int sure_k = kBins - 1, sure_p = kBins - 1, prob_p = kBins - 2, may_p = kBins - 1, fit = -1;
-#pragma unroll
-        for (int j = 3; j >= 0; --j) {
-          const int bin = lane * 4 + j;
-          if (bin >= kBins - 1) continue;
-          if (ci - cnt + c4[j] >= (unsigned int)k) sure_k = bin;
-          if (li - low + l4[j] >= want * kListMargin) sure_p = bin;
-          if (mi - mid + m4[j] >= likely) prob_p = bin;
-          if (hi - high + h4[j] >= want / kListMargin) may_p = bin;
-          if (ci - cnt + c4[j] <= (unsigned int)kList) fit = max(fit, bin);
-        }
-        sure_k = __reduce_min_sync(0xffffffffu, sure_k);
-        sure_p = __reduce_min_sync(0xffffffffu, sure_p);
-        prob_p = __reduce_min_sync(0xffffffffu, prob_p);
-        may_p = __reduce_min_sync(0xffffffffu, may_p);
-        fit = __reduce_max_sync(0xffffffffu, fit);
-        if (lane == 0) {
-          sel[0] = sure_k;
-          sel[1] = sure_p;
-          sel[2] = may_p;
-          // one bin more than the one that holds the cut; a list that turns out short of the mass is given up again
-          sel[3] = cut_k ? (sure_k + 1 <= fit ? sure_k + 1 : -1) : min(prob_p + 1, fit);
-        }
-      }
-      __syncthreads();
-      const int last_bin = sel[3];
-      bool listed = last_bin >= 0;
-      if (listed) {
-        // ------------------------------------------------ few tokens: collect, sort, walk
-        for (int w = tid; w < s.nw; w += kThreads)
-          s.each(w, [&](float v, int i) {
-            const float lw = rs.log_weight(v);
-            if (lw > -(kBins - 1) / 8.f && (int)(lw * -8.f) <= last_bin)
-              keys[atomicAdd(&n_list, 1u)] = rank_key(v, i);
-          });
-        __syncthreads();
-        const unsigned int mine = n_list;
-        if (CL > 1) {
-          nvb::cluster_sync();
-          if (rank == 0) {  // gather behind the own ones
-            unsigned int at = mine;
-            for (uint32_t q = 1; q < CL; ++q) {
-              const unsigned int n = peer_load(&n_list, q);
-              for (unsigned int i = tid; i < n; i += kThreads) keys[at + i] = peer_load(&keys[i], q);
-              at += n;
-            }
-            if (tid == 0) slot_n = at;
+      threshold = threshold_sh;
+      for (int w = tid; w < s.nw; w += kThreads)
+        s.each(w, [&](float v, int i) {
+          if (v >= threshold && v > -INFINITY) {
+            const unsigned int at = atomicAdd(&n_list, 1u);
+            if (at < (unsigned int)kOwnList) keys[at] = rank_key(v, i);
           }
-        } else if (tid == 0) {
-          slot_n = mine;
+        });
+    }
+    Z = sum1((double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]));
+    if (cuts) {
+      // (the sum was a barrier of the cluster)
+      const unsigned int own_n = (uint32_t)lane < CL ? peer_load(&n_list, lane) : 0u;
+      threshold = nvb::warp_max((uint32_t)lane < CL ? peer_load(&threshold_sh, lane) : -INFINITY);
+      // a top_k is among the tokens at or above the largest threshold, of which there are top_k; for a top_p that is seen
+      bool listed = !__any_sync(0xffffffffu, own_n > (unsigned int)kOwnList) && (!cut_k || k <= want_top);
+      if (listed && rank == 0) {
+        // ------------------------------------------------------------ few tokens: gather, rank, walk
+        unsigned long long* list = reinterpret_cast<unsigned long long*>(pool);
+        double* sorted = pool + kList;
+        const uint32_t sure = order_key(threshold + 0.f);  // the list is complete down to here
+        for (uint32_t q = warp; q < CL; q += kWarps) {
+          const unsigned int nq = __shfl_sync(0xffffffffu, own_n, q);
+          for (unsigned int i = lane; i < nq; i += 32) {
+            const unsigned long long key = peer_load(&keys[i], q);
+            if ((uint32_t)(key >> 32) >= sure) {
+              const unsigned int at = atomicAdd(&n_gather, 1u);
+              if (at < (unsigned int)kList) list[at] = key;
+            }
+          }
         }
         __syncthreads();
-        if (rank == 0) {
-          const int n = (int)slot_n;
-          int n2 = 32;
-          while (n2 < n) n2 *= 2;
-          for (int i = n + tid; i < n2; i += kThreads) keys[i] = 0;
-          __syncthreads();
-          for (int size = 2; size <= n2; size *= 2)
-            for (int d = size / 2; d > 0; d /= 2) {
-              for (int i = tid; i < n2 / 2; i += kThreads) {
-                const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
-                const bool down = (lo & size) == 0;
-                const unsigned long long p = keys[lo], q = keys[hi];
-                if ((p < q) == down) {
-                  keys[lo] = q;
-                  keys[hi] = p;
-                }
-              }
-              __syncthreads();
-            }
-          // weights in order, two tokens per thread, and the sums before each
-          const int nk = cut_k ? min(k, n) : n;
-          double w2[2], sum = 0.0;
+        const int n = (int)n_gather;
+        listed = n <= kList;
+        if (listed) {
+          // a token's place is the number of larger keys
+          constexpr int OWN = kList / kThreads;
+          unsigned long long key[OWN];
+          int place[OWN];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int i = tid * 2 + j;
-            w2[j] = i < nk ? rs.weight64(key_logit(keys[i]), table) : 0.0;
-            sum += w2[j];
+          for (int o = 0; o < OWN; ++o) {
+            const int i = tid + o * kThreads;
+            key[o] = i < n ? list[i] : 0;
+            place[o] = 0;
+            if (i < n)
+#pragma unroll 4
+              for (int j = 0; j < n; ++j) place[o] += list[j] > key[o];
+          }
+          __syncthreads();
+#pragma unroll
+          for (int o = 0; o < OWN; ++o)
+            if (tid + o * kThreads < n) {
+              list[place[o]] = key[o];
+              sorted[place[o]] = rs.weight64(key_logit(key[o]), table);
+            }
+          __syncthreads();
+          // sums before each, consecutive places in a thread
+          const int nk = cut_k ? min(k, n) : n;
+          double w[OWN], sum = 0.0;
+#pragma unroll
+          for (int o = 0; o < OWN; ++o) {
+            w[o] = tid * OWN + o < nk ? sorted[tid * OWN + o] : 0.0;
+            sum += w[o];
           }
           double incl = sum;
 #pragma unroll
@@ -509,222 +560,282 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
             all += sh_d[i];
           }
           const double want = cut_p ? (double)top * (cut_k ? all : Z) : 4.0 * kMaxVocab;
-          listed = cut_k || all >= want;  // with a token of each bin behind the cut's, roundings of the weights included
+          listed = cut_k || all >= want;
           double before = base + incl - sum, kept = 0.0;
           int last = -1;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int i = tid * 2 + j;
+          for (int o = 0; o < OWN; ++o) {
+            const int i = tid * OWN + o;
             if (i < nk && (i == 0 || before < want)) {
               last = i;
-              kept += w2[j];
+              kept += w[o];
             }
-            before += w2[j];
+            before += w[o];
           }
           last = __reduce_max_sync(0xffffffffu, last);
-          if (lane == 0) sh_i[warp] = last;
-          kept = block_sum(kept, sh_d);
-          for (int i = 0; i < kWarps; ++i) last = max(last, sh_i[i]);
-          if (tid == 0) {
-            cut_sh = keys[last];
-            z_sh = kept;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
+          __syncthreads();
+          if (lane == 0) {
+            sh_i[warp] = last;
+            sh_d[warp] = kept;
           }
           __syncthreads();
           if (listed) {
-            cut = cut_sh;
-            Z = z_sh;
+            Z = 0.0;
+            for (int i = 0; i < kWarps; ++i) {
+              last = max(last, sh_i[i]);
+              Z += sh_d[i];
+            }
+            cut = list[last];
           }
-          if (tid == 0) sel_u[0] = listed;
-          __syncthreads();
-        }
-        if (CL > 1 && !cut_k) {
-          nvb::cluster_sync();
-          listed = peer_load(&sel_u[0], 0) != 0;
-          nvb::cluster_sync();
         }
       }
-      if (!listed) {
-        // ------------------------------------------------ many: radix select over the tokens whose logits lie in the
-        // range of those in the bins in question
+      unsigned long long told[1] = {rank == 0 && listed ? 1ull : 0ull};
+      cluster_reduce<1, true>(told, red, turn);
+      if (told[0] == 0) {
+        // ------------------------------------------------------------ many: counts by 1/16 octave of weight bound the
+        // cut; its logit by quartering the range of the logits in the bins in question, then its token among the equals
         auto bin_of = [&](float v) {
-          const float lw = rs.log_weight(v);
-          return lw > -(kBins - 1) / 8.f ? (int)(lw * -8.f) : kBins - 1;
+          const float lw = simple ? rs.log_weight_simple(v) : rs.log_weight(v);
+          return lw > -(kBins - 1) / kPerOctave ? (int)(lw * -kPerOctave) : kBins - 1;
         };
-        // sum of 1 or of the masses over f(logit, token)
-        auto total_of = [&](bool by_mass, unsigned long long* slot, auto f) {
-          unsigned long long n = 0;
-          for (int w = tid; w < s.nw; w += kThreads)
-            s.each(w, [&](float v, int i) {
-              if (i >= s.lo && i < s.hi && f(v, i)) n += by_mass ? (unsigned long long)(rs.weight(v) * kUnit) : 1ull;
-            });
-          return cluster_sum(n, sh_u, slot);
-        };
-        int flip = 0;
-        // the smallest kept key when 1 or masses are summed in descending key order up to ``target``, of the keys >= floor
-        auto select = [&](bool by_mass, unsigned long long target, int from, int upto, unsigned long long floor_key,
-                          int slot) {
-          float lo = -INFINITY, hi = -INFINITY;  // -smallest and largest logit
-          for (int w = tid; w < s.nw; w += kThreads)
-            s.each(w, [&](float v, int i) {
-              const int bin = bin_of(v);
-              if (bin < from || bin > upto || i < s.lo || i >= s.hi) return;
-              v = fmaxf(v, -INFINITY);
-              lo = fmaxf(lo, -v);
-              hi = fmaxf(hi, v);
-            });
-          lo = -cluster_max(lo, sh_f, &slot_f3[slot][0]);
-          hi = cluster_max(hi, sh_f, &slot_f3[slot][1]);
-          unsigned long long before = total_of(by_mass, &slot_u[slot * 2 + 1], [&](float v, int i) {
-            return v > hi && rank_key(v, i) >= floor_key;
+        for (int w = tid; w < s.nw; w += kThreads)
+          s.each(w, [&](float v, int) {
+            const int bin = bin_of(v);
+            if (bin < kBins - 1) atomicAdd(&hist[bin], 1u);
           });
-          // bits that differ: of the logits, then of the tokens
-          const uint32_t diff = order_key(lo + 0.f) ^ order_key(hi + 0.f);
-          const int token_bits = 32 - __clz(V - 1);
-          int bits = diff != 0 ? 64 - __clz(diff) : token_bits;
-          const unsigned long long top_key = (unsigned long long)order_key(hi + 0.f) << 32 | 0xffffffffull;
-          unsigned long long prefix = bits < 64 ? top_key >> bits << bits : 0ull;
-          while (bits > 0) {
-            const int nb = min(8, bits > 32 ? bits - 32 : bits), shift = bits - nb;
-            const unsigned int bin_mask = (1u << nb) - 1;
-            unsigned long long* h = hist_m[flip];
-            unsigned int* hc = hist_c[flip];
-            if (tid < 256) h[tid] = 0, hc[tid] = 0;
-            __syncthreads();
-            for (int w = tid; w < s.nw; w += kThreads)
-              s.each(w, [&](float v, int i) {
-                if (!(v <= hi) && !isnan(v)) return;
-                if (v < lo || i < s.lo || i >= s.hi) return;
-                const unsigned long long key = rank_key(v, i);
-                if (key < floor_key || (bits < 64 ? (key ^ prefix) >> bits : 0ull) != 0) return;
-                const unsigned int bin = (unsigned int)(key >> shift) & bin_mask;
-                atomicAdd(&hc[bin], 1u);
-                if (by_mass) atomicAdd(&h[bin], (unsigned long long)(rs.weight(v) * kUnit));
-              });
-            __syncthreads();
-            if (CL > 1) nvb::cluster_sync();
-            // every CTA adds up the cluster's bins and finds the same one
-            if (tid < 256) {
-              unsigned long long v = 0;
-              unsigned int c = 0;
-              for (uint32_t i = 0; i < CL; ++i) {
-                c += CL > 1 ? peer_load(&hc[tid], i) : hc[tid];
-                if (by_mass) v += CL > 1 ? peer_load(&h[tid], i) : h[tid];
-              }
-              keys[tid] = by_mass ? v : c;
-              keys[256 + tid] = c;
-            }
-            __syncthreads();
-            if (warp == 0) {  // lane: 8 bins from the top
-              unsigned long long own = 0;
+        nvb::cluster_sync();
+        if (tid < kBins) {
+          unsigned int n = 0;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) own += keys[255 - lane * 8 - i];
-              unsigned long long incl = own;
+          for (int i = 0; i < kMaxCluster; ++i) n += (uint32_t)i < CL ? peer_load(&hist[tid], i) : 0u;
+          hist_all[tid] = n;
+        }
+        __syncthreads();
+        if (warp == 0) {
+          // lane: 8 bins.  Counts, and the lowest and highest mass that they allow, from the largest weights on
+          constexpr int PL = kBins / 32;
+          unsigned int cnt = 0, c[PL];
+          float low = 0.f, high = 0.f, l[PL], h[PL];
+#pragma unroll
+          for (int j = 0; j < PL; ++j) {
+            const int bin = lane * PL + j;
+            const unsigned int n = bin < kBins - 1 ? hist_all[bin] : 0u;
+            c[j] = cnt += n;
+            l[j] = low += n * exp2f((bin + 1.01f) / -kPerOctave);
+            h[j] = high += n * exp2f((bin - 0.01f) / -kPerOctave);
+          }
+          unsigned int ci = cnt;
+          float li = low, hi = high;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned int cu = __shfl_up_sync(0xffffffffu, ci, o);
+            const float lu = __shfl_up_sync(0xffffffffu, li, o), hu = __shfl_up_sync(0xffffffffu, hi, o);
+            if (lane >= o) ci += cu, li += lu, hi += hu;
+          }
+          const float want = (float)((double)top * Z);
+          // first bin that certainly / possibly reaches the target
+          int sure_k = kBins - 1, sure_p = kBins - 1, may_p = kBins - 1;
+#pragma unroll
+          for (int j = PL - 1; j >= 0; --j) {
+            const int bin = lane * PL + j;
+            if (bin >= kBins - 1) continue;
+            if (ci - cnt + c[j] >= (unsigned int)k) sure_k = bin;
+            if (li - low + l[j] >= want * kSlack) sure_p = bin;
+            if (hi - high + h[j] >= want / kSlack) may_p = bin;
+          }
+          sure_k = __reduce_min_sync(0xffffffffu, sure_k);
+          sure_p = __reduce_min_sync(0xffffffffu, sure_p);
+          may_p = __reduce_min_sync(0xffffffffu, may_p);
+          if (lane == 0) sel[0] = sure_k, sel[1] = sure_p, sel[2] = may_p;
+        }
+        __syncthreads();
+        const int sure_k = sel[0], sure_p = sel[1], may_p = sel[2];
+        constexpr int SH = sizeof(T) == 2 ? 16 : 0;  // bits of the order that the type does not have
+        auto value_of = [](uint32_t key) {           // a negative number's missing bits are ones in the order
+          uint32_t k32 = key << SH;
+          if (SH > 0 && k32 < 0x80000000u) k32 |= (1u << SH) - 1;
+          return key_logit((unsigned long long)k32 << 32);
+        };
+        float* range = reinterpret_cast<float*>(pool);
+        constexpr int kRange = 4 * kList;
+        // the smallest kept key when 1 or weights are summed in descending order up to ``target``, of the keys >= floor
+        auto select = [&](bool by_mass, double target, int from, int upto, unsigned long long floor_key, int slot) {
+          const float floor_v = floor_key != 0 ? key_logit(floor_key) : -INFINITY;
+          const int floor_i = floor_key != 0 ? (int)(0xffffffffu - (uint32_t)floor_key) : 0x7fffffff;
+          auto one_of = [&](float v) {
+            return !by_mass ? 1.f : exp2f(simple ? rs.log_weight_simple(v) : rs.log_weight(v));
+          };
+          // the bins before ``from`` are kept; the logits of those in question go to ``range`` when they fit
+          float ends[3] = {-INFINITY, -INFINITY, 0.f};  // -smallest and largest logit, their number
+          double above = 0.0;
+          for (int w = tid; w < s.nw; w += kThreads) {
+            float part = 0.f;
+            s.each(w, [&](float v, int i) {
+              if (!(v > -INFINITY) || v < floor_v || (v == floor_v && i > floor_i)) return;
+              const int bin = bin_of(v);
+              if (bin < from) part += one_of(v);
+              if (bin < from || bin > upto) return;
+              ends[0] = fmaxf(ends[0], -v);
+              ends[1] = fmaxf(ends[1], v);
+              const unsigned int at = atomicAdd(&n_range[slot], 1u);
+              if (at < (unsigned int)kRange) range[at] = v;
+            });
+            above += part;
+          }
+          __syncthreads();
+          const int n_own = (int)n_range[slot];
+          ends[2] = (float)n_own;
+          cluster_reduce<3, true>(ends, red, turn);
+          above = sum1(above);
+          const float lo_v = -ends[0], hi_v = ends[1];
+          const bool fits = ends[2] <= (float)kRange;
+          // sums over the logits in question at or above each of three (``strict``: above)
+          auto sums = [&](const float (&t)[3], bool strict, double (&out)[3]) {
+            float acc[3] = {0.f, 0.f, 0.f};
+            double all[3] = {0.0, 0.0, 0.0};
+            auto add = [&](float v) {
+              const float one = one_of(v);
+#pragma unroll
+              for (int q = 0; q < 3; ++q) acc[q] += v > t[q] || (v == t[q] && !strict) ? one : 0.f;
+            };
+            if (fits) {
+              for (int i = tid; i < n_own; i += kThreads) add(range[i]);
+            } else {
+              int since = 0;
+              for (int w = tid; w < s.nw; w += kThreads) {
+                s.each(w, [&](float v, int i) {
+                  if (v >= lo_v && v <= hi_v && (v > floor_v || (v == floor_v && i <= floor_i))) add(v);
+                });
+                if (++since == 4) {  // at most 32 terms in 32 bits
+                  since = 0;
+#pragma unroll
+                  for (int q = 0; q < 3; ++q) all[q] += acc[q], acc[q] = 0.f;
+                }
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < 3; ++q) out[q] = all[q] + acc[q];
+            cluster_reduce<3, false>(out, red, turn);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) out[q] += above;
+          };
+          // the sum at lo reaches the target, the one above hi does not
+          uint32_t lo = order_key(lo_v + 0.f) >> SH, hi = order_key(hi_v + 0.f) >> SH;
+          while (lo < hi) {
+            const uint32_t n = hi - lo;  // thresholds in (lo, hi]
+            const uint32_t k1 = lo + (n + 3) / 4, k2 = lo + (n + 1) / 2, k3 = lo + (uint32_t)((3ull * n + 3) / 4);
+            const float t[3] = {value_of(k1), value_of(k2), value_of(k3)};
+            double f[3];
+            sums(t, false, f);
+            if (f[2] >= target) lo = k3;
+            else if (f[1] >= target) lo = k2, hi = k3 - 1;
+            else if (f[0] >= target) lo = k1, hi = k2 - 1;
+            else hi = k1 - 1;
+          }
+          const float v_cut = value_of(lo);
+          const float t[3] = {v_cut, v_cut, v_cut};
+          double f[3];
+          sums(t, true, f);
+          const double missing = ceil((target - f[0]) / fmax((double)one_of(v_cut), 1e-300));
+          const int n_keep = (int)fmin(fmax(missing, 1.0), 2.0 * kMaxVocab);
+          // the n_keep lowest tokens among the equal ones: counts of consecutive words, in token order
+          const int per = (s.nw + kWarps - 1) / kWarps, w0 = min(s.nw, warp * per), w1 = min(s.nw, w0 + per);
+          auto equals = [&](int w) {
+            int n = 0;
+            s.each(w, [&](float v, int i) { n += v == v_cut && i >= s.lo && i < s.hi; });
+            return n;
+          };
+          int n = 0;
+          for (int w = w0 + lane; w < w1; w += 32) n += equals(w);
+          n = __reduce_add_sync(0xffffffffu, n);
+          if ((uint32_t)lane < CL) peer_store(&eq_sh[slot][rank * kWarps + warp], lane, (unsigned int)n);
+          nvb::cluster_sync();
+          int before = 0;
+          for (int i = lane; i < (int)rank * kWarps + warp; i += 32) before += (int)eq_sh[slot][i];
+          before = __reduce_add_sync(0xffffffffu, before);
+          if (before < n_keep && before + n >= n_keep) {  // the last kept one is in this warp's words
+            for (int wb = w0; wb < w1; wb += 32) {
+              const int mine = wb + lane < w1 ? equals(wb + lane) : 0;
+              int incl = mine;
 #pragma unroll
               for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += v;
+                const int y = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += y;
               }
-              const unsigned hit = __ballot_sync(0xffffffffu, before + incl >= target);
-              if (lane == (hit != 0 ? __ffs(hit) - 1 : 31)) {
-                unsigned long long cum = before + incl - own;
-                int bin = 255 - lane * 8;
-                for (; bin > 248 - lane * 8 && cum + keys[bin] < target; --bin) cum += keys[bin];
-                sel_u[0] = prefix & ~(((unsigned long long)bin_mask) << shift) | ((unsigned long long)bin << shift);
-                sel_u[1] = cum;
-                sel[1] = keys[256 + bin] <= 1;
+              if (before + incl - mine < n_keep && before + incl >= n_keep) {
+                int left = n_keep - (before + incl - mine);
+                s.each(wb + lane, [&](float v, int i) {
+                  if (v == v_cut && i >= s.lo && i < s.hi && --left == 0) found_sh[slot] = rank_key(v, i);
+                });
               }
+              before += __shfl_sync(0xffffffffu, incl, 31);
             }
-            __syncthreads();
-            prefix = sel_u[0] >> shift << shift;
-            before = sel_u[1];
-            const bool alone = sel[1] != 0;
-            bits = shift;
-            if (bits == 32 && token_bits < 32) {  // token bits above the vocabulary's are ones
-              bits = token_bits;
-              prefix |= 0xffffffffull >> token_bits << token_bits;
-            }
-            flip ^= 1;  // the peers may still read the other one
-            __syncthreads();
-            if (alone) break;  // no other key begins like this
           }
-          return prefix;
+          __syncthreads();
+          unsigned long long found[1] = {found_sh[slot]};  // when all equal ones stay nobody has it
+          cluster_reduce<1, true>(found, red, turn);
+          return found[0] != 0 ? found[0] : (unsigned long long)order_key(v_cut + 0.f) << 32;
         };
-        const int sure_k = sel[0], sure_p = sel[1], may_p = sel[2];
-        __syncthreads();
-        if (cut_k) cut = select(false, (unsigned long long)k, max(0, sure_k - 1), min(kBins - 1, sure_k + 1), 0, 0);
+        auto kept_mass = [&] {
+          double z = 0.0;
+          for (int w = tid; w < s.nw; w += kThreads) {
+            float part = 0.f;
+            s.each(w, [&](float v, int i) {
+              if (cut == 0 || rank_key(v, i) >= cut) part += rs.weight(v);
+            });
+            z += part;
+          }
+          return sum1(z);
+        };
+        if (cut_k) {
+          cut = select(false, (double)k, max(0, sure_k - 1), min(kBins - 1, sure_k + 1), 0, 0);
+          Z = kept_mass();
+        }
         if (cut_p) {
-          const unsigned long long total =
-              total_of(true, &slot_u[0], [&](float v, int i) { return rank_key(v, i) >= cut; });
-          const double want = (double)total * (double)top;
-          const unsigned long long target = want > 1.0 ? (unsigned long long)ceil(want) : 1ull;  // the first always stays
-          cut = max(cut, select(true, target, cut_k ? 0 : max(0, may_p - 1), cut_k ? kBins - 1 : min(kBins - 1, sure_p + 1),
-                                cut, 1));
+          cut = max(cut, select(true, (double)top * Z, cut_k ? 0 : max(0, may_p - 1),
+                                cut_k ? kBins - 1 : min(kBins - 1, sure_p + 1), cut, 1));
+          Z = kept_mass();
         }
-        double z = 0.0;
-        for (int w = tid; w < s.nw; w += kThreads) {
-          float part = 0.f;
-          s.each(w, [&](float v, int i) {
-            if (rank_key(v, i) >= cut) part += rs.weight(v);
-          });
-          z += part;
-        }
-        Z = cluster_sum(z, sh_d, &slot_d[1]);
       }
     }
   }
-  if (rank == 0 && tid == 0) {
+  if (rank != 0) return;  // (no CTA touches another's shared memory behind the last barrier)
+  if (tid == 0) {
     a.cut[r] = cut;
     a.row_max[r] = m;
   }
-  if (r + 1 < rows.y) {  // the draft
-    bool near = false;
-    double w = 0.0, uq = 0.0;
-    if (rank == 0) {
-      const int dr = a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
-      const long d = a.ids[r + 1];
-      if (a.probs != nullptr && dr >= a.D) {
-        if (tid == 0) nvb::record_error(a.err, nvb::kErrBadArgument);
-      } else if (d >= 0 && d < V) {
-        const float v = to_float(x[d]);
-        if (rank_key(v, (int)d) >= cut) w = rs.weight64(v, table);
-        uq = a.uniform(r) * (a.probs != nullptr ? (double)a.probs[dr * a.probs_ld + d] : 1.0);
+  if (drafted) {
+    const double w = d >= 0 && rank_key(d_logit, (int)d) >= cut ? rs.weight64(d_logit, table) : 0.0;
+    if (w > 0.0 && fabs(uq * Z - w) <= 1e-4 * w) {  // too near for a sum of 32-bit weights: the row once more
+      double z = 0.0;
+      for (int i = tid; i < V; i += kThreads) {
+        const float v = to_float(x[i]);
+        if (rank_key(v, i) >= cut) z += rs.weight64(v, table);
       }
-      near = fabs(uq * Z - w) <= 1e-4 * w;  // too near for a sum of 32-bit weights
-      if (tid == 0) sel[0] = near;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      __syncthreads();
+      if (lane == 0) sh_d[warp] = z;
+      __syncthreads();
+      Z = 0.0;
+      for (int i = 0; i < kWarps; ++i) Z += sh_d[i];
     }
-    if (CL > 1) {
-      nvb::cluster_sync();
-      near = peer_load(&sel[0], 0) != 0;
-      if (near) cut = rank == 0 ? cut : 0;  // only rank 0 needs to know the cut from here
-    }
-    if (near) {
-      if (CL > 1) {
-        if (rank == 0 && tid == 0) sel_u[0] = cut;
-        nvb::cluster_sync();
-        cut = peer_load(&sel_u[0], 0);
-      }
-      double z64 = 0.0;
-      for (int q = tid; q < s.nw; q += kThreads)
-        s.each(q, [&](float v, int i) {
-          if (rank_key(v, i) >= cut && i >= s.lo && i < s.hi) z64 += rs.weight64(v, table);
-        });
-      Z = cluster_sum(z64, sh_d, &slot_d[2]);
-    }
-    if (rank == 0 && tid == 0) a.accept[r] = uq * Z < w;
+    if (tid == 0) a.accept[r] = uq * Z < w;
   }
-  if (CL > 1) nvb::cluster_sync();  // nobody leaves while its shared memory may be read
 }
 
 // One cluster per sequence: the accepted drafts and the drawn token.  Weights and sums in 64 bits: the token depends on
 // which side of a sum the uniform falls, and a row has as many sums as tokens.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyArgs a) {
   nvb::pdl_wait();
   nvb::pdl_trigger();
   extern __shared__ __align__(128) uint8_t buf[];
   __shared__ uint64_t bar;
-  __shared__ double sh_d[32], slot_d, table[kTable], warp_sum_sh[2][kWarps], all_sh[kMaxCluster * kWarps + 1];
-  __shared__ int sh_i[32];
+  __shared__ double red[2][3][kMaxCluster * kWarps], table[kTable], all_sh[2][kMaxCluster * kWarps + 1];
+  __shared__ int sh_i[kWarps];
   const int b = blockIdx.x / cluster_size(), tid = threadIdx.x, V = a.V, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
   const int2 rows = seq_rows(a, b);
@@ -740,6 +851,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
     }
     return;
   }
+  cluster_arrive();
   int acc = n - 1;  // accepted drafts: up to the first refusal
   for (int j0 = 0; j0 < n - 1; j0 += 32) {
     const bool no = j0 + lane < n - 1 && !a.accept[rows.x + j0 + lane];
@@ -759,6 +871,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
   const long drafted = rejected && a.probs == nullptr ? a.ids[r + 1] : -1;
   fill_table(table);
   finish_slice(s, &bar, a.err);
+  cluster_wait();
   const bool simple = cut == 0 && rs.simple();
   const float cut_logit = cut == 0 ? -INFINITY : key_logit(cut);
   constexpr int PER = Slice<T>::PER;
@@ -785,7 +898,10 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
 #pragma unroll
       for (int j = 0; j < PER; ++j) z += l[j];
     }
-    const double Z = cluster_sum(z, sh_d, &slot_d);
+    double zs[1] = {z};
+    int turn = 0;
+    cluster_reduce<1, false>(zs, red, turn);
+    const double Z = zs[0];
     Zinv = Z > 0.0 ? 1.0 / Z : 0.0;
   }
   const bool q_aligned = q != nullptr && ((reinterpret_cast<uintptr_t>(q) + 4 * (long)s.first) & 15) == 0;
@@ -825,35 +941,33 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) warp_sum_sh[plain][warp] = sum;
-    __syncthreads();
-    if (CL > 1) nvb::cluster_sync();
-    // sums before each warp of the cluster, in token order; every CTA computes the same ones
+    // every warp's sum to every CTA: the sums before each warp of the cluster, in token order, the same everywhere
+    if ((uint32_t)lane < CL) peer_store(&all_sh[plain][rank * kWarps + warp], lane, sum);
+    nvb::cluster_sync();
     const int nws = (int)CL * kWarps;
-    if (tid < nws) all_sh[tid] = CL > 1 ? peer_load(&warp_sum_sh[plain][tid % kWarps], tid / kWarps) : warp_sum_sh[plain][tid];
-    __syncthreads();
+    double* all = all_sh[plain];
     if (tid == 0) {
       double c = 0.0;  // one after the other: the sums never decrease
       for (int i = 0; i < nws; i += kWarps) {
         double v[kWarps];
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) v[k] = all_sh[i + k];
+        for (int k = 0; k < kWarps; ++k) v[k] = all[i + k];
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) {
-          all_sh[i + k] = c;
+          all[i + k] = c;
           c += v[k];
         }
       }
-      all_sh[nws] = c;
+      all[nws] = c;
     }
     __syncthreads();
-    const double total = all_sh[nws];
+    const double total = all[nws];
     if (total > 0.0) {
       // below total whatever the uniform is, so some token exceeds it
       const double want = fmin(fmax(a.uniform(rows.y - 1), 0.0), 1.0 - 2.220446049250313e-16) * total;
       const int me = (int)rank * kWarps + warp;
-      double c = all_sh[me];
-      if (c <= want && all_sh[me + 1] > want) {  // this warp's words hold it
+      double c = all[me];
+      if (c <= want && all[me + 1] > want) {  // this warp's words hold it
         int tok = -1;
         for (int wb = w0; wb < w1; wb += 32) {
           double mine = 0.0;
@@ -895,7 +1009,6 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs 
       if (j != acc) out[j] = j < acc ? a.ids[rows.x + j + 1] : -1;
     if (tid == 0) a.counts[b] = acc + 1;
   }
-  if (CL > 1) nvb::cluster_sync();  // nobody leaves while its shared memory may be read
 }
 
 }  // namespace
@@ -962,10 +1075,10 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   const bool wide = logits.scalar_type() == at::kFloat;
   const int64_t width = wide ? 4 : 2;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // CTAs per row: two of them fit an SM (their slices at most 80 KB), more while SMs would idle
+  // CTAs per row: four of them fit an SM (their slices at most 44 KB), more while SMs would idle
   auto cluster_for = [&](int64_t count) {
     int64_t n = 1;
-    while (n < kMaxCluster && (V * width > n * 80 * 1024 || count * n * 2 <= sms)) n *= 2;
+    while (n < kMaxCluster && (V * width > n * 44 * 1024 || count * n * 2 <= sms)) n *= 2;
     return n;
   };
   auto run = [&](auto kern, int64_t count) {
