@@ -27,13 +27,10 @@ using bf16 = __nv_bfloat16;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr double kLog2e64 = 1.4426950408889634074;
 constexpr int kMaxVocab = 327680;  // 32-bit logits of a row in the shared memory of eight CTAs
-constexpr int kMaxCluster = 8;
-constexpr int kBins = 256;   // of 1/16 octave of weight below the row's largest; the last one holds the rest
-constexpr float kPerOctave = 16.f;
+constexpr int kMaxCluster = 16;
 constexpr int kList = 256;     // tokens that a cut is found among by ranking
-constexpr int kOwnList = 128;  // of one CTA
+constexpr int kOwnList = 256;  // of one CTA
 constexpr int kTop = 64;     // largest top_k that the list is tried for
-constexpr float kSlack = 1.0001f;  // of sums of 32-bit weights
 
 struct VerifyArgs {
   const void* logits;
@@ -178,34 +175,47 @@ NV_DEVICE void peer_store(T* p, uint32_t rank, T v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(*reinterpret_cast<uint32_t*>(&v)) : "memory");
 }
 
-// Reductions over the cluster with one barrier: every warp writes its values into every CTA's table, each thread then
-// reads its own CTA's, in the same order everywhere.  Two tables in turn: whoever writes one again has passed a barrier
-// that everybody reached after reading it.
+// Reductions over the cluster with one barrier of it: the CTAs' totals go into every CTA's table, each thread then reads
+// its own CTA's, in the same order everywhere.  Two tables in turn: whoever writes one again has passed a barrier that
+// everybody reached after reading it.
+constexpr int kValues = 6;
+struct Tables {
+  double v[2][kValues][kMaxCluster], warps[kValues][kWarps];
+};
 template <int N, bool MAX, typename T>
-NV_DEVICE void cluster_reduce(T (&v)[N], double (&tables)[2][3][kMaxCluster * kWarps], int& turn) {
-  constexpr int STRIDE = kMaxCluster * kWarps;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t n = cluster_size(), rank = nvb::cluster_ctarank();
-  T* t = reinterpret_cast<T*>(tables[turn & 1]);
+NV_DEVICE void cluster_reduce(T (&v)[N], Tables& tables, int& turn) {
+  static_assert(N <= kValues && N * kMaxCluster <= kThreads);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = (int)cluster_size(), rank = (int)nvb::cluster_ctarank();
+  T* t = reinterpret_cast<T*>(tables.v[turn & 1]);
+  T* sh = reinterpret_cast<T*>(tables.warps);
   ++turn;
   auto join = [](T a, T b) { return MAX ? (a > b ? a : b) : a + b; };
 #pragma unroll
   for (int k = 0; k < N; ++k) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[k] = join(v[k], __shfl_xor_sync(0xffffffffu, v[k], o));
-    if ((uint32_t)lane < n) peer_store(&t[k * STRIDE + rank * kWarps + warp], lane, v[k]);
+    if (lane == 0) sh[k * kWarps + warp] = v[k];
+  }
+  __syncthreads();
+  if (tid < N * n) {
+    const int k = tid / n, peer = tid % n;
+    T x = sh[k * kWarps];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) x = join(x, sh[k * kWarps + w]);
+    peer_store(&t[k * kMaxCluster + rank], peer, x);
   }
   nvb::cluster_sync();
-  const int entries = (int)n * kWarps;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    T x = lane < entries ? t[k * STRIDE + lane] : (MAX ? v[k] : (T)0);
-    if (lane + 32 < entries) x = join(x, t[k * STRIDE + lane + 32]);
+    T x = t[k * kMaxCluster + (lane < n ? lane : 0)];
+    if (lane >= n && !MAX) x = (T)0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x = join(x, __shfl_xor_sync(0xffffffffu, x, o));
     v[k] = x;
   }
 }
+
 // The cluster's CTAs are there once each has arrived: waited for before the first access to another's shared memory.
 NV_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 NV_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
@@ -323,15 +333,14 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   nvb::pdl_trigger();
   extern __shared__ __align__(128) uint8_t buf[];
   __shared__ uint64_t bar;
-  __shared__ double red[2][3][kMaxCluster * kWarps], table[kTable], sh_d[kWarps];
+  __shared__ Tables red;
+  __shared__ double table[kTable], sh_d[kWarps];
   __shared__ float sh_f[kWarps], threshold_sh;
-  __shared__ int sh_i[kWarps], sel[3];
-  __shared__ unsigned int hist[kBins], n_list, n_gather, n_range[2], eq_sh[2][kMaxCluster * kWarps];
+  __shared__ int sh_i[kWarps];
+  __shared__ unsigned int n_list, n_gather, eq_sh[2][kMaxCluster * kWarps];
   __shared__ unsigned long long keys[kOwnList], found_sh[2];
-  // the threads' maxima, then rank 0's list (keys, and weights in order), then the row's bins, then the logits in question
-  __shared__ __align__(16) double pool[2 * kList];
+  __shared__ double pool[2 * kList];  // the threads' maxima, then rank 0's list: keys, and weights in order
   float* maxima = reinterpret_cast<float*>(pool);
-  unsigned int* hist_all = reinterpret_cast<unsigned int*>(pool);
   const int r = blockIdx.x / cluster_size(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
   cluster_arrive();
@@ -367,9 +376,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
     }
   }
   fill_table(table);
-  for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
   if (tid == 0) {
-    n_list = n_gather = n_range[0] = n_range[1] = 0;
+    n_list = n_gather = 0;
     found_sh[0] = found_sh[1] = 0;
   }
   finish_slice(s, &bar, a.err);
@@ -398,28 +406,28 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
     } else if (mc == INFINITY) {
       for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { z4[0] += v == INFINITY ? 1.f : 0.f; });
     }
-    // warps' sums and the CTA's maximum to every CTA
+    // the CTAs' sums and maxima to every CTA
     double z = (double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    if ((uint32_t)lane < CL) {
-      peer_store(&red[0][0][rank * kWarps + warp], lane, z);
-      peer_store(&red[0][1][rank * kWarps + warp], lane, (double)mc);
+    if (lane == 0) sh_d[warp] = z;
+    __syncthreads();
+    if (tid < (int)CL) {
+      z = 0.0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) z += sh_d[i];
+      peer_store(&red.v[0][0][rank], tid, z);
+      peer_store(&red.v[0][1][rank], tid, (double)mc);
     }
     turn = 1;
     nvb::cluster_sync();
-    float mx = -INFINITY;
-    for (int i = lane; i < (int)CL * kWarps; i += 32) mx = fmaxf(mx, (float)red[0][1][i]);
-    m = nvb::warp_max(mx);
-    const RowScale rs(m, 0.f, temp);
-    double t = 0.0;
-    for (int i = lane; i < (int)CL * kWarps; i += 32) {
-      const double zi = red[0][0][i];
-      if (zi > 0.0) t += zi * rs.weight64((float)red[0][1][i], table);
-    }
+    const float ml = lane < (int)CL ? (float)red.v[0][1][lane] : -INFINITY;
+    const double zl = lane < (int)CL ? red.v[0][0][lane] : 0.0;
+    m = nvb::warp_max(ml);
+    const RowScale all(m, 0.f, temp);
+    Z = zl > 0.0 ? zl * all.weight64(ml, table) : 0.0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    Z = t;
+    for (int o = 16; o > 0; o >>= 1) Z += __shfl_xor_sync(0xffffffffu, Z, o);
   } else {
     float mv[1] = {mine_max};
     cluster_reduce<1, true>(mv, red, turn);
@@ -440,9 +448,9 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   } else if (cut_k || cut_p || a.softcap > 0.f) {
     const bool cuts = (cut_k || cut_p) && m != -INFINITY;
     // With a cut: this CTA's tokens at or above its threshold, the want_top-th largest of its threads' maxima, so at least
-    // that many; the row's list holds every token at or above the largest threshold of the cluster.  A top_k needs
-    // top_k of them in case one CTA has them all, a top_p some 256 in the cluster.
-    const int want_top = cut_k ? min(k, kTop) : max(32, min(128, 256 / (int)CL));
+    // that many; the row's list holds every token at or above the largest threshold of the cluster.  That is enough for a
+    // top_k when it holds top_k tokens (two times as many are aimed at), for a top_p when it holds the mass.
+    const int want_top = min(128, (cut_k ? 2 * min(k, kTop) : 160) / (int)CL + 8);
     if (cuts) {
       maxima[tid] = mine_max;
       __syncthreads();
@@ -494,20 +502,23 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
     Z = sum1((double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]));
     if (cuts) {
       // (the sum was a barrier of the cluster)
-      const unsigned int own_n = (uint32_t)lane < CL ? peer_load(&n_list, lane) : 0u;
-      threshold = nvb::warp_max((uint32_t)lane < CL ? peer_load(&threshold_sh, lane) : -INFINITY);
-      // a top_k is among the tokens at or above the largest threshold, of which there are top_k; for a top_p that is seen
-      bool listed = !__any_sync(0xffffffffu, own_n > (unsigned int)kOwnList) && (!cut_k || k <= want_top);
-      if (listed && rank == 0) {
-        // ------------------------------------------------------------ few tokens: gather, rank, walk
+      constexpr double kAll = 4.0 * kMaxVocab;  // more than any count or mass
+      // Rank 0: the CTAs' lists as far as they hold logits in [from, to) (to NaN: no end) and keys >= floor, ranked and
+      // walked, behind ``count`` tokens of the mass ``mass``.  Kept are the first ``limit`` tokens, while the mass before
+      // is below ``want`` (negative: below that share of the mass that the limit leaves).  False when the list is too long
+      // or, unless it is ``certain`` to hold the cut, ends before it.
+      auto walk = [&](float from, float to, unsigned long long floor_key, double count, double mass, double limit,
+                      double want, bool certain) {
         unsigned long long* list = reinterpret_cast<unsigned long long*>(pool);
         double* sorted = pool + kList;
-        const uint32_t sure = order_key(threshold + 0.f);  // the list is complete down to here
+        const unsigned int own_n = (uint32_t)lane < CL ? peer_load(&n_list, lane) : 0u;
+        if (__any_sync(0xffffffffu, own_n > (unsigned int)kOwnList)) return false;
         for (uint32_t q = warp; q < CL; q += kWarps) {
           const unsigned int nq = __shfl_sync(0xffffffffu, own_n, q);
           for (unsigned int i = lane; i < nq; i += 32) {
             const unsigned long long key = peer_load(&keys[i], q);
-            if ((uint32_t)(key >> 32) >= sure) {
+            const float v = key_logit(key);
+            if (v >= from && !(v >= to) && key >= floor_key) {
               const unsigned int at = atomicAdd(&n_gather, 1u);
               if (at < (unsigned int)kList) list[at] = key;
             }
@@ -515,198 +526,89 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         }
         __syncthreads();
         const int n = (int)n_gather;
-        listed = n <= kList;
-        if (listed) {
-          // a token's place is the number of larger keys
-          constexpr int OWN = kList / kThreads;
-          unsigned long long key[OWN];
-          int place[OWN];
-#pragma unroll
-          for (int o = 0; o < OWN; ++o) {
-            const int i = tid + o * kThreads;
-            key[o] = i < n ? list[i] : 0;
-            place[o] = 0;
-            if (i < n)
+        if (n > kList) return false;
+        // a token's place is the number of larger keys
+        static_assert(kList == kThreads);
+        const unsigned long long key = tid < n ? list[tid] : 0;
+        int place = 0;
+        if (tid < n)
 #pragma unroll 4
-              for (int j = 0; j < n; ++j) place[o] += list[j] > key[o];
-          }
-          __syncthreads();
-#pragma unroll
-          for (int o = 0; o < OWN; ++o)
-            if (tid + o * kThreads < n) {
-              list[place[o]] = key[o];
-              sorted[place[o]] = rs.weight64(key_logit(key[o]), table);
-            }
-          __syncthreads();
-          // sums before each, consecutive places in a thread
-          const int nk = cut_k ? min(k, n) : n;
-          double w[OWN], sum = 0.0;
-#pragma unroll
-          for (int o = 0; o < OWN; ++o) {
-            w[o] = tid * OWN + o < nk ? sorted[tid * OWN + o] : 0.0;
-            sum += w[o];
-          }
-          double incl = sum;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-          }
-          if (lane == 31) sh_d[warp] = incl;
-          __syncthreads();
-          double base = 0.0, all = 0.0;
-          for (int i = 0; i < kWarps; ++i) {
-            if (i < warp) base += sh_d[i];
-            all += sh_d[i];
-          }
-          const double want = cut_p ? (double)top * (cut_k ? all : Z) : 4.0 * kMaxVocab;
-          listed = cut_k || all >= want;
-          double before = base + incl - sum, kept = 0.0;
-          int last = -1;
-#pragma unroll
-          for (int o = 0; o < OWN; ++o) {
-            const int i = tid * OWN + o;
-            if (i < nk && (i == 0 || before < want)) {
-              last = i;
-              kept += w[o];
-            }
-            before += w[o];
-          }
-          last = __reduce_max_sync(0xffffffffu, last);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
-          __syncthreads();
-          if (lane == 0) {
-            sh_i[warp] = last;
-            sh_d[warp] = kept;
-          }
-          __syncthreads();
-          if (listed) {
-            Z = 0.0;
-            for (int i = 0; i < kWarps; ++i) {
-              last = max(last, sh_i[i]);
-              Z += sh_d[i];
-            }
-            cut = list[last];
-          }
+          for (int j = 0; j < n; ++j) place += list[j] > key;
+        __syncthreads();
+        if (tid < n) {
+          list[place] = key;
+          sorted[place] = count + place < limit ? rs.weight64(key_logit(key), table) : 0.0;
         }
-      }
-      unsigned long long told[1] = {rank == 0 && listed ? 1ull : 0ull};
+        __syncthreads();
+        const double w = tid < n ? sorted[tid] : 0.0;
+        double incl = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        if (lane == 31) sh_d[warp] = incl;
+        __syncthreads();
+        double base = mass, all = mass;
+        for (int i = 0; i < kWarps; ++i) {
+          if (i < warp) base += sh_d[i];
+          all += sh_d[i];
+        }
+        const bool enough = certain || (limit < kAll ? count + n >= limit : all >= want);
+        if (want < 0.0) want = -want * all;
+        const bool keep = tid < n && count + tid < limit && (base + incl - w < want || count + tid == 0.0);
+        const int kept = __popc(__ballot_sync(0xffffffffu, keep));  // the kept ones are the first
+        double kw = keep ? w : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) kw += __shfl_xor_sync(0xffffffffu, kw, o);
+        __syncthreads();
+        if (lane == 0) {
+          sh_i[warp] = kept;
+          sh_d[warp] = kw;
+        }
+        __syncthreads();
+        int last = -1;
+        double z = mass;
+        for (int i = 0; i < kWarps; ++i) {
+          last += sh_i[i];
+          z += sh_d[i];
+        }
+        if (!enough || last < 0) return false;
+        cut = list[last];
+        Z = z;
+        return true;
+      };
+      threshold = nvb::warp_max((uint32_t)lane < CL ? peer_load(&threshold_sh, lane) : -INFINITY);
+      bool done = false;
+      if (rank == 0 && (!cut_k || k <= kTop))  // the lists are complete down to the largest threshold
+        done = walk(threshold, NAN, 0, 0.0, 0.0, cut_k ? (double)k : kAll,
+                    !cut_p ? kAll : cut_k ? -(double)top : (double)top * Z, false);
+      unsigned long long told[1] = {rank == 0 && done ? 1ull : 0ull};
       cluster_reduce<1, true>(told, red, turn);
       if (told[0] == 0) {
-        // ------------------------------------------------------------ many: counts by 1/16 octave of weight bound the
-        // cut; its logit by quartering the range of the logits in the bins in question, then its token among the equals
-        auto bin_of = [&](float v) {
-          const float lw = simple ? rs.log_weight_simple(v) : rs.log_weight(v);
-          return lw > -(kBins - 1) / kPerOctave ? (int)(lw * -kPerOctave) : kBins - 1;
-        };
-        for (int w = tid; w < s.nw; w += kThreads)
-          s.each(w, [&](float v, int) {
-            const int bin = bin_of(v);
-            if (bin < kBins - 1) atomicAdd(&hist[bin], 1u);
-          });
-        nvb::cluster_sync();
-        if (tid < kBins) {
-          unsigned int n = 0;
-#pragma unroll
-          for (int i = 0; i < kMaxCluster; ++i) n += (uint32_t)i < CL ? peer_load(&hist[tid], i) : 0u;
-          hist_all[tid] = n;
-        }
-        __syncthreads();
-        if (warp == 0) {
-          // lane: 8 bins.  Counts, and the lowest and highest mass that they allow, from the largest weights on
-          constexpr int PL = kBins / 32;
-          unsigned int cnt = 0, c[PL];
-          float low = 0.f, high = 0.f, l[PL], h[PL];
-#pragma unroll
-          for (int j = 0; j < PL; ++j) {
-            const int bin = lane * PL + j;
-            const unsigned int n = bin < kBins - 1 ? hist_all[bin] : 0u;
-            c[j] = cnt += n;
-            l[j] = low += n * exp2f((bin + 1.01f) / -kPerOctave);
-            h[j] = high += n * exp2f((bin - 0.01f) / -kPerOctave);
-          }
-          unsigned int ci = cnt;
-          float li = low, hi = high;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const unsigned int cu = __shfl_up_sync(0xffffffffu, ci, o);
-            const float lu = __shfl_up_sync(0xffffffffu, li, o), hu = __shfl_up_sync(0xffffffffu, hi, o);
-            if (lane >= o) ci += cu, li += lu, hi += hu;
-          }
-          const float want = (float)((double)top * Z);
-          // first bin that certainly / possibly reaches the target
-          int sure_k = kBins - 1, sure_p = kBins - 1, may_p = kBins - 1;
-#pragma unroll
-          for (int j = PL - 1; j >= 0; --j) {
-            const int bin = lane * PL + j;
-            if (bin >= kBins - 1) continue;
-            if (ci - cnt + c[j] >= (unsigned int)k) sure_k = bin;
-            if (li - low + l[j] >= want * kSlack) sure_p = bin;
-            if (hi - high + h[j] >= want / kSlack) may_p = bin;
-          }
-          sure_k = __reduce_min_sync(0xffffffffu, sure_k);
-          sure_p = __reduce_min_sync(0xffffffffu, sure_p);
-          may_p = __reduce_min_sync(0xffffffffu, may_p);
-          if (lane == 0) sel[0] = sure_k, sel[1] = sure_p, sel[2] = may_p;
-        }
-        __syncthreads();
-        const int sure_k = sel[0], sure_p = sel[1], may_p = sel[2];
-        constexpr int SH = sizeof(T) == 2 ? 16 : 0;  // bits of the order that the type does not have
-        auto value_of = [](uint32_t key) {           // a negative number's missing bits are ones in the order
-          uint32_t k32 = key << SH;
-          if (SH > 0 && k32 < 0x80000000u) k32 |= (1u << SH) - 1;
-          return key_logit((unsigned long long)k32 << 32);
-        };
-        float* range = reinterpret_cast<float*>(pool);
-        constexpr int kRange = 4 * kList;
-        // the smallest kept key when 1 or weights are summed in descending order up to ``target``, of the keys >= floor
-        auto select = [&](bool by_mass, double target, int from, int upto, unsigned long long floor_key, int slot) {
-          const float floor_v = floor_key != 0 ? key_logit(floor_key) : -INFINITY;
-          const int floor_i = floor_key != 0 ? (int)(0xffffffffu - (uint32_t)floor_key) : 0x7fffffff;
-          auto one_of = [&](float v) {
-            return !by_mass ? 1.f : exp2f(simple ? rs.log_weight_simple(v) : rs.log_weight(v));
-          };
-          // the bins before ``from`` are kept; the logits of those in question go to ``range`` when they fit
-          float ends[3] = {-INFINITY, -INFINITY, 0.f};  // -smallest and largest logit, their number
-          double above = 0.0;
-          for (int w = tid; w < s.nw; w += kThreads) {
-            float part = 0.f;
-            s.each(w, [&](float v, int i) {
-              if (!(v > -INFINITY) || v < floor_v || (v == floor_v && i > floor_i)) return;
-              const int bin = bin_of(v);
-              if (bin < from) part += one_of(v);
-              if (bin < from || bin > upto) return;
-              ends[0] = fmaxf(ends[0], -v);
-              ends[1] = fmaxf(ends[1], v);
-              const unsigned int at = atomicAdd(&n_range[slot], 1u);
-              if (at < (unsigned int)kRange) range[at] = v;
-            });
-            above += part;
-          }
-          __syncthreads();
-          const int n_own = (int)n_range[slot];
-          ends[2] = (float)n_own;
-          cluster_reduce<3, true>(ends, red, turn);
-          above = sum1(above);
-          const float lo_v = -ends[0], hi_v = ends[1];
-          const bool fits = ends[2] <= (float)kRange;
-          // sums over the logits in question at or above each of three (``strict``: above)
-          auto sums = [&](const float (&t)[3], bool strict, double (&out)[3]) {
+        // ------------------------------------------------------------ beyond the list: the range of logits that holds the
+        // cut is quartered until few tokens are left in it, or one logit
+        // The smallest kept key when 1 or weights are summed in descending order up to ``target``, of the keys >= floor;
+        // leaves the kept mass in Z when weights are summed.
+        auto select = [&](bool by_mass, double target, float lo, unsigned long long floor_key, int slot) {
+          float hi = INFINITY;  // the cut's logit is in [lo, hi), while not ``open`` in [lo, m]
+          bool open = false;
+          double over[2] = {0.0, 0.0};  // sum and count from hi on
+          double in_lo = kAll;          // count from lo on
+          // sums and counts of the logits at or above each of three
+          auto sums = [&](const float (&t)[3], double (&out)[6]) {
             float acc[3] = {0.f, 0.f, 0.f};
+            int cnt[3] = {0, 0, 0};
             double all[3] = {0.0, 0.0, 0.0};
-            auto add = [&](float v) {
-              const float one = one_of(v);
+            auto pass = [&](auto one_of) {
+              for (int w = tid, since = 0; w < s.nw; w += kThreads) {
+                s.each(w, [&](float v, int) {
+                  const float one = one_of(v);
 #pragma unroll
-              for (int q = 0; q < 3; ++q) acc[q] += v > t[q] || (v == t[q] && !strict) ? one : 0.f;
-            };
-            if (fits) {
-              for (int i = tid; i < n_own; i += kThreads) add(range[i]);
-            } else {
-              int since = 0;
-              for (int w = tid; w < s.nw; w += kThreads) {
-                s.each(w, [&](float v, int i) {
-                  if (v >= lo_v && v <= hi_v && (v > floor_v || (v == floor_v && i <= floor_i))) add(v);
+                  for (int q = 0; q < 3; ++q) {
+                    acc[q] += v >= t[q] ? one : 0.f;
+                    cnt[q] += v >= t[q];
+                  }
                 });
                 if (++since == 4) {  // at most 32 terms in 32 bits
                   since = 0;
@@ -714,33 +616,91 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
                   for (int q = 0; q < 3; ++q) all[q] += acc[q], acc[q] = 0.f;
                 }
               }
+            };
+            if (!by_mass) pass([](float) { return 0.f; });
+            else if (simple) pass([&](float v) { return exp2f(rs.log_weight_simple(v)); });
+            else pass([&](float v) { return rs.weight(v); });
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+              out[3 + q] = (double)cnt[q];
+              out[q] = by_mass ? all[q] + acc[q] : (double)cnt[q];
             }
-#pragma unroll
-            for (int q = 0; q < 3; ++q) out[q] = all[q] + acc[q];
-            cluster_reduce<3, false>(out, red, turn);
-#pragma unroll
-            for (int q = 0; q < 3; ++q) out[q] += above;
+            cluster_reduce<6, false>(out, red, turn);
           };
-          // the sum at lo reaches the target, the one above hi does not
-          uint32_t lo = order_key(lo_v + 0.f) >> SH, hi = order_key(hi_v + 0.f) >> SH;
-          while (lo < hi) {
-            const uint32_t n = hi - lo;  // thresholds in (lo, hi]
-            const uint32_t k1 = lo + (n + 3) / 4, k2 = lo + (n + 1) / 2, k3 = lo + (uint32_t)((3ull * n + 3) / 4);
-            const float t[3] = {value_of(k1), value_of(k2), value_of(k3)};
-            double f[3];
-            sums(t, false, f);
-            if (f[2] >= target) lo = k3;
-            else if (f[1] >= target) lo = k2, hi = k3 - 1;
-            else if (f[0] >= target) lo = k1, hi = k2 - 1;
-            else hi = k1 - 1;
+          // the next larger logit (denormals count as zero)
+          auto next_up = [](float v) {
+            if (fabsf(v) < FLT_MIN) return FLT_MIN;
+            const float n = key_logit((unsigned long long)(order_key(v) + 1) << 32);
+            return fabsf(n) < FLT_MIN ? 0.f : n;
+          };
+          const float eps = sizeof(T) == 2 ? 0.00390625f : 1.1920929e-7f;  // half a step, a step of the type
+          float one_logit = NAN;
+          for (int step = 0; step < 300; ++step) {
+            const bool few = in_lo - over[1] <= (double)kList;
+            const float top_v = open ? hi : m;
+            const bool narrow = top_v - lo <= eps * fmaxf(fabsf(top_v), fabsf(lo)) || step % 8 == 7;
+            if (few || narrow) {  // the smallest and largest logit that are left
+              float ends[2] = {-INFINITY, -INFINITY};
+              for (int w = tid; w < s.nw; w += kThreads)
+                s.each(w, [&](float v, int) {
+                  const bool in = v >= lo && (open ? v < hi : v <= m) && v > -INFINITY;
+                  ends[0] = fmaxf(ends[0], in ? -v : -INFINITY);
+                  ends[1] = fmaxf(ends[1], in ? v : -INFINITY);
+                });
+              cluster_reduce<2, true>(ends, red, turn);
+              if (!(-ends[0] < ends[1])) {
+                one_logit = ends[1];
+                break;
+              }
+              if (few) break;
+              lo = -ends[0];
+              if (ends[1] < INFINITY) hi = next_up(ends[1]), open = true;
+            }
+            // Three logits between; any of them splits the range.  Equal parts of it, or of the order while it is wide.
+            const float up = open ? hi : m, span = 0.25f * up - 0.25f * lo;
+            float t[3] = {lo + span, lo + 2.f * span, up - span};
+            if (!(up - lo <= 64.f * (1.f + fabsf(m)))) {
+              const uint32_t kl = order_key(lo + 0.f), part = (order_key(up + 0.f) - kl) / 4;
+#pragma unroll
+              for (int q = 0; q < 3; ++q) t[q] = key_logit((unsigned long long)(kl + (q + 1) * part) << 32);
+            }
+            if (!(t[0] > lo)) t[0] = t[1] = t[2] = next_up(lo);
+            double f[6];
+            sums(t, f);
+            if (f[2] >= target) lo = t[2], in_lo = f[5];
+            else {
+              if (f[1] >= target) lo = t[1], in_lo = f[4], hi = t[2], over[0] = f[2], over[1] = f[5];
+              else if (f[0] >= target) lo = t[0], in_lo = f[3], hi = t[1], over[0] = f[1], over[1] = f[4];
+              else hi = t[0], over[0] = f[0], over[1] = f[3];
+              open = true;
+            }
           }
-          const float v_cut = value_of(lo);
-          const float t[3] = {v_cut, v_cut, v_cut};
-          double f[3];
-          sums(t, true, f);
-          const double missing = ceil((target - f[0]) / fmax((double)one_of(v_cut), 1e-300));
+          if (isnan(one_logit)) {  // few tokens: as above
+            if (tid == 0) n_list = n_gather = 0;
+            __syncthreads();
+            for (int w = tid; w < s.nw; w += kThreads)
+              s.each(w, [&](float v, int i) {
+                if (v >= lo && (!open || v < hi) && v > -INFINITY && i >= s.lo && i < s.hi) {
+                  const unsigned int at = atomicAdd(&n_list, 1u);
+                  if (at < (unsigned int)kOwnList) keys[at] = rank_key(v, i);
+                }
+              });
+            nvb::cluster_sync();
+            if (rank == 0)
+              walk(lo, open ? hi : NAN, floor_key, over[1], by_mass ? over[0] : 0.0, by_mass ? kAll : target,
+                   by_mass ? target : kAll, true);
+            unsigned long long c[1] = {rank == 0 ? cut : 0ull};
+            cluster_reduce<1, true>(c, red, turn);
+            double z[1] = {rank == 0 && tid == 0 ? Z : 0.0};
+            cluster_reduce<1, false>(z, red, turn);
+            Z = z[0];
+            return c[0];
+          }
+          // many equal logits: the n_keep lowest tokens among them, by counts of consecutive words, in token order
+          const float v_cut = one_logit;
+          const double one = by_mass ? (double)rs.weight(v_cut) : 1.0;
+          const double missing = ceil((target - over[0]) / fmax(one, 1e-300));
           const int n_keep = (int)fmin(fmax(missing, 1.0), 2.0 * kMaxVocab);
-          // the n_keep lowest tokens among the equal ones: counts of consecutive words, in token order
           const int per = (s.nw + kWarps - 1) / kWarps, w0 = min(s.nw, warp * per), w1 = min(s.nw, w0 + per);
           auto equals = [&](int w) {
             int n = 0;
@@ -776,27 +736,30 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
           __syncthreads();
           unsigned long long found[1] = {found_sh[slot]};  // when all equal ones stay nobody has it
           cluster_reduce<1, true>(found, red, turn);
+          double all_eq = 0.0;
+          for (int i = lane; i < (int)CL * kWarps; i += 32) all_eq += (double)eq_sh[slot][i];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) all_eq += __shfl_xor_sync(0xffffffffu, all_eq, o);
+          Z = over[0] + one * fmin((double)n_keep, all_eq);
           return found[0] != 0 ? found[0] : (unsigned long long)order_key(v_cut + 0.f) << 32;
         };
-        auto kept_mass = [&] {
+        if (cut_k) {
+          cut = select(false, (double)k, -FLT_MAX, 0, 0);
           double z = 0.0;
           for (int w = tid; w < s.nw; w += kThreads) {
             float part = 0.f;
             s.each(w, [&](float v, int i) {
-              if (cut == 0 || rank_key(v, i) >= cut) part += rs.weight(v);
+              if (rank_key(v, i) >= cut) part += rs.weight(v);
             });
             z += part;
           }
-          return sum1(z);
-        };
-        if (cut_k) {
-          cut = select(false, (double)k, max(0, sure_k - 1), min(kBins - 1, sure_k + 1), 0, 0);
-          Z = kept_mass();
+          Z = sum1(z);
         }
         if (cut_p) {
-          cut = max(cut, select(true, (double)top * Z, cut_k ? 0 : max(0, may_p - 1),
-                                cut_k ? kBins - 1 : min(kBins - 1, sure_p + 1), cut, 1));
-          Z = kept_mass();
+          const unsigned long long floor_key = cut;
+          // below the largest by log V + 18 temperatures all tokens together weigh less than 2^-25
+          const float lo = simple ? fmaxf(m - temp * (logf((float)V) + 18.f), -FLT_MAX) : -FLT_MAX;
+          cut = max(floor_key, select(true, (double)top * Z, cut_k ? key_logit(cut) : lo, floor_key, 1));
         }
       }
     }
@@ -834,7 +797,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   nvb::pdl_trigger();
   extern __shared__ __align__(128) uint8_t buf[];
   __shared__ uint64_t bar;
-  __shared__ double red[2][3][kMaxCluster * kWarps], table[kTable], all_sh[2][kMaxCluster * kWarps + 1];
+  __shared__ Tables red;
+  __shared__ double table[kTable], all_sh[2][kMaxCluster * kWarps + 1];
   __shared__ int sh_i[kWarps];
   const int b = blockIdx.x / cluster_size(), tid = threadIdx.x, V = a.V, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
@@ -1075,17 +1039,18 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   const bool wide = logits.scalar_type() == at::kFloat;
   const int64_t width = wide ? 4 : 2;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // CTAs per row: four of them fit an SM (their slices at most 44 KB), more while SMs would idle
+  // CTAs per row: four of them fit an SM (their slices at most 44 KB), up to 8 while SMs would idle, 16 (beyond the
+  // portable size) for rows that 8 would hold in larger slices
   auto cluster_for = [&](int64_t count) {
     int64_t n = 1;
-    while (n < kMaxCluster && (V * width > n * 44 * 1024 || count * n * 2 <= sms)) n *= 2;
+    while (n < kMaxCluster && (V * width > n * 44 * 1024 || (n < 8 && count * n * 2 <= sms))) n *= 2;
     return n;
   };
   auto run = [&](auto kern, int64_t count) {
     const int64_t n = cluster_for(count);
     const size_t smem = (size_t)(((V + n - 1) / n + 7) / 8 * 8 * width + 32);
-    TORCH_CHECK(smem <= 190 * 1024, "the vocabulary does not fit the shared memory of a cluster");
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (n > 8) C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     C10_CUDA_CHECK(nvb::launch_cluster(kern, dim3((unsigned)(n * count)), dim3(kThreads), smem, stream, (unsigned)n, a));
   };
   if (R > 0) {
