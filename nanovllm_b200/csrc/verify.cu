@@ -476,7 +476,9 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
       }
     }
     float z4[4] = {0.f, 0.f, 0.f, 0.f};
-    if (simple) {
+    if (cuts && cut_k) {
+      // the mass of all tokens is not asked for
+    } else if (simple) {
       for (int w = tid; w < s.nw; w += kThreads) {
         int j = 0;
         s.each(w, [&](float v, int) { z4[j++ & 3] += exp2f(rs.log_weight_simple(v)); });
@@ -798,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   extern __shared__ __align__(128) uint8_t buf[];
   __shared__ uint64_t bar;
   __shared__ Tables red;
-  __shared__ double table[kTable], all_sh[2][kMaxCluster * kWarps + 1];
+  __shared__ double table[kTable], all_sh[2][kMaxCluster * kWarps + 1], sub_sh[kWarps];
   __shared__ int sh_i[kWarps];
   const int b = blockIdx.x / cluster_size(), tid = threadIdx.x, V = a.V, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
@@ -839,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   const bool simple = cut == 0 && rs.simple();
   const float cut_logit = cut == 0 ? -INFINITY : key_logit(cut);
   constexpr int PER = Slice<T>::PER;
-  // weights of a word's tokens (what a slice's first and last word hold besides weighs nothing)
+  // weights of a word's tokens (what a slice's first and last word hold besides weighs nothing); false: nothing
   auto word_weights = [&](int w, double (&l)[PER]) {
     const uint4 raw = reinterpret_cast<const uint4*>(s.words)[w];
     const T* e = reinterpret_cast<const T*>(&raw);
@@ -847,18 +849,23 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
 #pragma unroll
       for (int j = 0; j < PER; ++j) l[j] = rs.weight64_simple(to_float(e[j]), table);
     } else {
+      bool any = false;  // with a cut most words lie below its logit
+#pragma unroll
+      for (int j = 0; j < PER; ++j) any |= to_float(e[j]) >= cut_logit;
+      if (!any) return false;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const float v = to_float(e[j]);  // with a cut most tokens are below its logit
+        const float v = to_float(e[j]);
         l[j] = v >= cut_logit && rank_key(v, s.first + w * PER + j) >= cut ? rs.weight64(v, table) : 0.0;
       }
     }
+    return true;
   };
   double Zinv = 1.0;
   if (q != nullptr) {  // p - q needs p itself
     double z = 0.0, l[PER];
     for (int w = tid; w < s.nw; w += kThreads) {
-      word_weights(w, l);
+      if (!word_weights(w, l)) continue;
 #pragma unroll
       for (int j = 0; j < PER; ++j) z += l[j];
     }
@@ -871,8 +878,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   const bool q_aligned = q != nullptr && ((reinterpret_cast<uintptr_t>(q) + 4 * (long)s.first) & 15) == 0;
   // what is left of a word's tokens to draw from; plain: the probabilities themselves
   auto word_left = [&](int w, bool plain, double (&l)[PER]) {
-    word_weights(w, l);
-    if (plain) return;
+    if (!word_weights(w, l)) return false;
+    if (plain) return true;
     const int i0 = s.first + w * PER;
     if (q == nullptr) {
 #pragma unroll
@@ -892,19 +899,23 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
 #pragma unroll
       for (int j = 0; j < PER; ++j) l[j] = l[j] > 0.0 ? fmax(0.0, l[j] * Zinv - (double)qv[j]) : 0.0;
     }
+    return true;
+  };
+  auto warp_left = [&](int wa, int wz, bool plain) {  // of words [wa, wz)
+    double sum = 0.0, l[PER];
+    for (int w = wa + lane; w < wz; w += 32)
+      if (word_left(w, plain, l))
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sum += l[j];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
   };
   // warps own consecutive words, lanes one word at a time
   const int per = (s.nw + kWarps - 1) / kWarps, w0 = min(s.nw, warp * per), w1 = min(s.nw, w0 + per);
   for (int plain = rejected ? 0 : 1; plain < 2; ++plain) {
     // plain: the probabilities themselves, also when nothing is left of p - q
-    double sum = 0.0, l[PER];
-    for (int w = w0 + lane; w < w1; w += 32) {
-      word_left(w, plain != 0, l);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) sum += l[j];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const double sum = warp_left(w0, w1, plain != 0);
     // every warp's sum to every CTA: the sums before each warp of the cluster, in token order, the same everywhere
     if ((uint32_t)lane < CL) peer_store(&all_sh[plain][rank * kWarps + warp], lane, sum);
     nvb::cluster_sync();
@@ -929,40 +940,56 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
     if (total > 0.0) {
       // below total whatever the uniform is, so some token exceeds it
       const double want = fmin(fmax(a.uniform(rows.y - 1), 0.0), 1.0 - 2.220446049250313e-16) * total;
-      const int me = (int)rank * kWarps + warp;
-      double c = all[me];
-      if (c <= want && all[me + 1] > want) {  // this warp's words hold it
-        int tok = -1;
-        for (int wb = w0; wb < w1; wb += 32) {
-          double mine = 0.0;
-          if (wb + lane < w1) {
-            word_left(wb + lane, plain != 0, l);
-#pragma unroll
-            for (int j = 0; j < PER; ++j) mine += l[j];
+      const double* ours = all + rank * kWarps;
+      if (ours[0] <= want && ours[kWarps] > want) {  // this CTA's words hold it: a warp's share of them, an eighth of that
+        int at = 0;
+        while (ours[at + 1] <= want) ++at;
+        const int wa = min(s.nw, at * per), wz = min(s.nw, wa + per), sub = (wz - wa + kWarps - 1) / kWarps;
+        const double part = warp_left(min(wz, wa + warp * sub), min(wz, wa + (warp + 1) * sub), plain != 0);
+        if (lane == 0) sub_sh[warp] = part;
+        __syncthreads();
+        if (warp == 0) {
+          // (sums in another order may end a rounding before ``want``: then it is the last token with weight)
+          double c = ours[at], c_last = c;
+          int k = 0, last = 0;
+          for (; k < kWarps; ++k) {
+            if (sub_sh[k] > 0.0) last = k, c_last = c;
+            if (c + sub_sh[k] > want) break;
+            c += sub_sh[k];
           }
-          double incl = mine;
+          if (k == kWarps) k = last, c = c_last;
+          int tok = -1;
+          const int wk = min(wz, wa + k * sub), we = min(wz, wk + sub);
+          for (int wb = wk; wb < we; wb += 32) {
+            double mine = 0.0, l[PER];
+            const bool some_here = wb + lane < we && word_left(wb + lane, plain != 0, l);
+            if (some_here)
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double v = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += v;
-          }
-          const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && c + incl > want);
-          const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
-          const int src = over != 0 ? __ffs(over) - 1 : some != 0 ? 31 - __clz(some) : -1;
-          int cand = -1;
-          if (lane == src) {
-            double d = c + incl - mine;
+              for (int j = 0; j < PER; ++j) mine += l[j];
+            double incl = mine;
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-              if (l[j] > 0.0 && !(cand >= 0 && d > want)) cand = s.first + (wb + lane) * PER + j;
-              d += l[j];
+            for (int o = 1; o < 32; o <<= 1) {
+              const double v = __shfl_up_sync(0xffffffffu, incl, o);
+              if (lane >= o) incl += v;
             }
+            const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && c + incl > want);
+            const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
+            const int src = over != 0 ? __ffs(over) - 1 : some != 0 ? 31 - __clz(some) : -1;
+            int cand = -1;
+            if (lane == src) {
+              double d = c + incl - mine;
+#pragma unroll
+              for (int j = 0; j < PER; ++j) {
+                if (l[j] > 0.0 && !(cand >= 0 && d > want)) cand = s.first + (wb + lane) * PER + j;
+                d += l[j];
+              }
+            }
+            if (src >= 0) tok = __shfl_sync(0xffffffffu, cand, src);
+            if (over != 0) break;
+            c += __shfl_sync(0xffffffffu, incl, 31);
           }
-          if (src >= 0) tok = __shfl_sync(0xffffffffu, cand, src);
-          if (over != 0) break;
-          c += __shfl_sync(0xffffffffu, incl, 31);
+          if (lane == 0) out[acc] = tok < 0 ? 0 : tok;
         }
-        if (lane == 0) out[acc] = tok < 0 ? 0 : tok;
       }
       break;
     }
