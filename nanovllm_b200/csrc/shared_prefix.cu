@@ -42,10 +42,17 @@ struct SpArgs {
   const int* ctx_lens;
   const int* cu_q;  // null: one token per sequence
   int B, T, nq, nkv, hd, block_size, num_blocks, max_q, max_len;
+  int G;              // query heads of a KV head
+  uint32_t g_magic;   // ceil(2^32 / G), 0 for G = 1
   float scale, softcap;
   int window;
   int* err;
 
+  // (f / G, f % G): the high word of f ceil(2^32 / G) is the quotient as long as f G < 2^32
+  NV_DEVICE int2 split(int f) const {
+    const int t = g_magic == 0 ? f : (int)__umulhi((uint32_t)f, g_magic);
+    return make_int2(t, f - t * G);
+  }
   NV_DEVICE int prefix_len() const { return prefix_len_dev != nullptr ? *prefix_len_dev : prefix_len_host; }
   NV_DEVICE bool prefix_ok(int P) const { return P >= 0 && (long)P <= (long)n_prefix_blocks * block_size; }
   // First and one-past-last query token of sequence b; an end before the first when cu_q or max_q do not fit.
@@ -155,13 +162,18 @@ struct SpPlan {
   NV_DEVICE int slots() const { return pre_slots + n_own; }
 };
 
-NV_DEVICE int sp_page(const SpArgs& a, const int* pages, int key) {
-  const int blk = pages[key / a.block_size];
+// A page number as the tables give it, or page 0 and an error.
+NV_DEVICE int sp_page(const SpArgs& a, int blk) {
   if (blk < 0 || blk >= a.num_blocks) {
     nvb::record_error(a.err, nvb::kErrBadArgument);
     return 0;
   }
   return blk;
+}
+// The page of tile ``tile`` (of ``keys`` keys) where the table has one.
+NV_DEVICE int sp_table(const SpArgs& a, const int* pages, int n_pages, int tile, int keys) {
+  const int at = (int)((long)tile * keys / a.block_size);
+  return at < n_pages ? pages[at] : -1;
 }
 
 // cu_q in shared memory (global beyond kCuSmem sequences): the search for a row's sequence is then free of
@@ -192,6 +204,8 @@ struct SpPart {
   int kvh, slot;
   int klo, kend, t0, t1;
   const int* pages;
+  int n_pages;
+  int page;  // in warp 0: the page of tile t0 + lane
 };
 
 // Four warps: RG groups of 16 rows times 4 / RG groups of 16 * RG keys of each tile.  S and O stay in registers
@@ -207,10 +221,16 @@ __device__ void sp_part_mma(const SpArgs& a, const SpPlan& pl, const SpPart& p, 
   constexpr bool kQRegs = HD <= 128;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c4 = lane & 3;
   const int rg = warp % RG, key0 = (warp / RG) * KW;
-  const int G = a.nq / a.nkv, nt = p.t1 - p.t0;
-  auto issue = [&](int i) {
+  const int G = a.G, nt = p.t1 - p.t0;
+  int page = p.page;
+  // Warp 0: the page of tile i, of which the lanes hold 32 at a time (a table look-up for each copy would come before it).
+  auto page_of = [&](int i) {
+    if (i >= 32 && (i & 31) == 0) page = sp_table(a, p.pages, p.n_pages, p.t0 + i + lane, KT);
+    return __shfl_sync(0xffffffffu, page, i & 31);
+  };
+  auto issue = [&](int i, int pg) {
     const int st = i % STAGES, tok = (p.t0 + i) * KT;
-    const int row = (sp_page(a, p.pages, tok) * a.nkv + p.kvh) * a.block_size + tok % a.block_size;
+    const int row = (sp_page(a, pg) * a.nkv + p.kvh) * a.block_size + tok % a.block_size;
     uint8_t* kd = ring + st * 2 * TILE;
     nvb::mbar_arrive_expect_tx(&bars[st], 2 * TILE);
 #pragma unroll
@@ -219,11 +239,14 @@ __device__ void sp_part_mma(const SpArgs& a, const SpPlan& pl, const SpPart& p, 
       nvb::tma_load_2d(kd + TILE + j * KT * 128, vmap, &bars[st], j * 64, row);
     }
   };
-  if (tid == 0)
-    for (int i = 0; i < STAGES && i < nt; ++i) issue(i);
+  if (warp == 0)
+    for (int i = 0; i < STAGES && i < nt; ++i) {
+      const int pg = page_of(i);
+      if (lane == 0) issue(i, pg);
+    }
   auto q_row = [&](int r) {
-    const int f = p.row0 + r;
-    return a.q + (long)(p.tok0 + f / G) * a.q_tok + (long)(p.kvh * G + f % G) * a.q_head;
+    const int2 f = a.split(p.row0 + r);
+    return a.q + (long)(p.tok0 + f.x) * a.q_tok + (long)(p.kvh * G + f.y) * a.q_head;
   };
   uint32_t qf[kQRegs ? HD / 16 : 1][4];
   if constexpr (kQRegs) {
@@ -358,7 +381,10 @@ __device__ void sp_part_mma(const SpArgs& a, const SpPlan& pl, const SpPart& p, 
       }
     }
     __syncthreads();
-    if (tid == 0 && i + STAGES < nt) issue(i + STAGES);
+    if (warp == 0 && i + STAGES < nt) {
+      const int pg = page_of(i + STAGES);
+      if (lane == 0) issue(i + STAGES, pg);
+    }
   }
   if (aborted) {  // reported in the error word; drain the copies still in flight (bounded)
     if (tid == 0)
@@ -372,8 +398,8 @@ __device__ void sp_part_mma(const SpArgs& a, const SpPlan& pl, const SpPart& p, 
   }
   const int NS = pl.slots();
   auto slot_of = [&](int r) {
-    const int f = p.row0 + r;
-    return ((long)(p.tok0 + f / G) * a.nq + p.kvh * G + f % G) * NS + p.slot;
+    const int2 f = a.split(p.row0 + r);
+    return ((long)(p.tok0 + f.x) * a.nq + p.kvh * G + f.y) * NS + p.slot;
   };
   if constexpr (RG == 4) {
 #pragma unroll
@@ -449,7 +475,7 @@ __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUten
   uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(qs) + (HD <= 128 ? 0 : kRows * (HD + 8) * 2));
   __shared__ int abort_flag, cu_sh[kCuSmem + 1], row_pos[kRows], pos_lo, pos_hi;
   const int tid = threadIdx.x;
-  const int G = a.nq / a.nkv, P = a.prefix_len();
+  const int G = a.G, P = a.prefix_len();
   const bool p_ok = a.prefix_ok(P);
   SpPart p{};
   int bid = blockIdx.x;
@@ -475,10 +501,12 @@ __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUten
     p.t0 = split * pl.pre_tiles;
     p.t1 = p.t0 + pl.pre_tiles;
     p.pages = a.prefix_blocks;
+    p.n_pages = a.n_prefix_blocks;
+    if (tid < 32) p.page = sp_table(a, p.pages, p.n_pages, p.t0 + tid, KT);
     const int* cu = stage_cu(a, cu_sh, 128);
     __syncthreads();
     if (tid < kRows && tid < p.rows) {
-      const int pos = row_position(a, cu, (p.row0 + tid) / G, P);
+      const int pos = row_position(a, cu, a.split(p.row0 + tid).x, P);
       row_pos[tid] = pos;
       if (pos >= 0) {
         atomicMin(&pos_lo, pos);
@@ -492,6 +520,10 @@ __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUten
     p.kvh = bid % a.nkv;
     bid /= a.nkv;
     const int b = bid / pl.own_row_tiles;
+    p.t0 = max(0, P) / KT + split * pl.own_tiles;
+    p.pages = a.block_tables + b * a.bt_stride;
+    p.n_pages = a.bt_width;
+    if (tid < 32) p.page = sp_table(a, p.pages, p.n_pages, p.t0 + tid, KT);  // (while the lengths are on their way)
     const int2 tk = a.tokens(b);
     const int ctx = a.ctx_lens[b], n = tk.y - tk.x;
     if (n < 0 || !p_ok || !a.ctx_ok(ctx, P)) {  // reported; the sequence's rows are undefined
@@ -505,12 +537,10 @@ __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUten
     p.slot = pl.pre_slots + split;
     p.klo = P;
     p.kend = ctx;
-    p.t0 = P / KT + split * pl.own_tiles;
     p.t1 = p.t0 + pl.own_tiles;
-    p.pages = a.block_tables + b * a.bt_stride;
     __syncthreads();
     if (tid < p.rows) {
-      const int pos = ctx - n + (p.row0 + tid) / G;
+      const int pos = ctx - n + a.split(p.row0 + tid).x;
       row_pos[tid] = pos;
       if (tid == 0) pos_lo = pos;
       if (tid == p.rows - 1) pos_hi = pos;
@@ -521,12 +551,15 @@ __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUten
   // only tiles that some row sees
   p.kend = min(p.kend, pos_hi + 1);
   p.t1 = p.kend > p.klo ? min(p.t1, (p.kend + KT - 1) / KT) : p.t0;
-  if (a.window > 0 && pos_lo != 0x7fffffff) p.t0 = max(p.t0, max(0, pos_lo - a.window + 1) / KT);
+  if (a.window > 0 && pos_lo != 0x7fffffff && max(0, pos_lo - a.window + 1) / KT > p.t0) {
+    p.t0 = max(0, pos_lo - a.window + 1) / KT;
+    if (tid < 32) p.page = sp_table(a, p.pages, p.n_pages, p.t0 + tid, KT);
+  }
   if (p.t0 >= p.t1) {
     const int NS = pl.slots();
     if (tid < p.rows) {
-      const int f = p.row0 + tid;
-      pl.part_lse[((long)(p.tok0 + f / G) * a.nq + p.kvh * G + f % G) * NS + p.slot] = -INFINITY;
+      const int2 f = a.split(p.row0 + tid);
+      pl.part_lse[((long)(p.tok0 + f.x) * a.nq + p.kvh * G + f.y) * NS + p.slot] = -INFINITY;
     }
     return;
   }
@@ -640,6 +673,29 @@ void split_keys(long groups, int tiles, long ctas, int* n, int* per) {
   *n = (tiles + *per - 1) / *per;
 }
 
+// How many splits the tcgen05 kernel takes of the prefix.  Its CTAs have an SM each to themselves and the own keys' kernel
+// runs on the others meanwhile, so the rule looks for the least time of the two together: a prefix CTA takes some 8 us and
+// 1.7 us for every key tile (two tiles when both its row tiles are the same rows); the own keys stream at 6 TB/s, which
+// two thirds of the SMs still reach.  (Measured with 32 and with 148 prefix CTAs: 32 sequences on 2048 keys 24 against
+// 34 us, 128 on 8192 keys 90 against 100 us, 96 on 16000 keys, narrow heads, 241 against 65 us.)
+void split_prefix(int groups, int tiles, bool twice, double own_bytes, int sms, int* n, int* per) {
+  const double own_us = own_bytes / 6.0e6;
+  double best = 1e30;
+  for (int splits = 1; splits <= tiles && (splits == 1 || (long)splits * groups <= sms); ++splits) {
+    const int each = (tiles + splits - 1) / splits;
+    const double waves = std::ceil((double)splits * groups / sms);
+    const double tc = waves * (8.0 + 1.7 * (twice ? (each + 1) / 2 : each));
+    const double share = std::min(1.0, 1.5 * std::max(0, sms - splits * groups) / sms);  // of the stream, meanwhile
+    const double total = own_us <= share * tc ? tc : tc + (own_us - share * tc);
+    if (total < best - 0.5) {  // parts are written and read again: more of them only where it shows
+      best = total;
+      *n = splits;
+      *per = each;
+    }
+  }
+  *n = (tiles + *per - 1) / *per;
+}
+
 void check_i32(const at::Tensor& t, const at::Tensor& like, int64_t dim, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.device() == like.device() &&
                   (t.size(-1) <= 1 || t.stride(-1) == 1),
@@ -690,7 +746,7 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
   TORCH_CHECK(max_q >= 1 && max_len >= 0 && window >= 0 && softcap >= 0.0, "max_q must be at least 1; max_len, window "
               "and softcap not negative");
   TORCH_CHECK(std::isfinite(scale) && std::isfinite(softcap), "scale and softcap must be finite");
-  TORCH_CHECK(max_len < (int64_t(1) << 30) && T * nq < (int64_t(1) << 30) && window < (int64_t(1) << 30),
+  TORCH_CHECK(max_len < (int64_t(1) << 30) && T * nq * (nq / nkv) < (int64_t(1) << 32) && T * nq < (int64_t(1) << 30) && window < (int64_t(1) << 30),
               "more keys or query rows than the kernels index");
   for (int64_t i = 0; i < 2; ++i)
     TORCH_CHECK(q.stride(i) % 8 == 0, "q rows must start on 16-byte boundaries");
@@ -728,6 +784,8 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
   a.B = (int)B, a.T = (int)T, a.nq = (int)nq, a.nkv = (int)nkv, a.hd = (int)hd;
   a.block_size = (int)bs, a.num_blocks = (int)NB, a.max_q = (int)max_q, a.max_len = (int)max_len;
   a.scale = (float)scale, a.softcap = (float)softcap, a.window = (int)window;
+  a.G = (int)(nq / nkv);
+  a.g_magic = a.G == 1 ? 0u : (uint32_t)(((uint64_t(1) << 32) + a.G - 1) / a.G);
   a.err = err.data_ptr<int>();
   auto stream = at::cuda::getCurrentCUDAStream();
   if (hd != 64 && hd != 128 && hd != 256) {
@@ -737,7 +795,7 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
                                reinterpret_cast<const bf16*>(v_cache.data_ptr())));
     return {out, 1};
   }
-  const int G = (int)(nq / nkv), sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int G = a.G, sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   const int64_t pre_bound = prefix_len_dev.has_value() ? prefix_blocks.numel() * bs : prefix_len;
   const int64_t pre_keys = std::min<int64_t>(pre_bound, max_len);
   const int own_tiles = (int)std::max<int64_t>(0, (max_len + KT - 1) / KT - (prefix_len_dev.has_value() ? 0 : prefix_len / KT));
@@ -746,10 +804,10 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
   pl.tc = pre_keys > 0 && hd <= 128 && bs % 128 == 0 && rows > 64;
   if (pl.tc) {
     pl.pre_row_tiles = (int)((rows + 255) / 256);
-    const int tiles = (int)((pre_keys + 127) / 128);
-    int n = std::max<int>(1, sms / (int)(nkv * pl.pre_row_tiles));
-    pl.pre_tiles = (tiles + n - 1) / n;
-    pl.n_pre = (tiles + pl.pre_tiles - 1) / pl.pre_tiles;
+    // half of the keys that the bound leaves to the sequences, on average
+    const double own_bytes = 2.0 * (double)(max_len - pre_keys) * (double)(B * nkv * hd);
+    split_prefix((int)(nkv * pl.pre_row_tiles), (int)((pre_keys + 127) / 128), rows <= 128, own_bytes, sms, &pl.n_pre,
+                 &pl.pre_tiles);
     pl.pre_slots = 2 * pl.n_pre;
   } else {
     pl.pre_row_tiles = (int)((rows + kRows - 1) / kRows);

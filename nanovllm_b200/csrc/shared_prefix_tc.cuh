@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
   nvb::pdl_wait();
   nvb::pdl_trigger();
 
-  const int G = a.nq / a.nkv, P = a.prefix_len();
+  const int G = a.G, P = a.prefix_len();
   int bid = blockIdx.x;
   const int split = bid % pl.n_pre;
   bid /= pl.n_pre;
@@ -219,22 +219,31 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
   int t0 = split * pl.pre_tiles;
   const int t1 = min(t0 + pl.pre_tiles, (kend + BN - 1) / BN);
   // one K or V tile into its ring
-  auto copy = [&](bool is_k, int i) {
+  auto copy = [&](bool is_k, int i, int pg) {
     const int s = i % (is_k ? KS : VS), tok = (t0 + i) * BN;
-    const int row = (sp_page(a, a.prefix_blocks, tok) * a.nkv + kvh) * a.block_size + tok % a.block_size;
+    const int row = (sp_page(a, pg) * a.nkv + kvh) * a.block_size + tok % a.block_size;
     uint8_t* dst = (is_k ? kring : vring) + (size_t)s * C::KTILE;
     uint64_t* bar = is_k ? &k_full[s] : &v_full[s];
     nvb::mbar_arrive_expect_tx(bar, C::KTILE);
 #pragma unroll
     for (int j = 0; j < HD / 64; ++j) nvb::tma_load_2d(dst + j * C::KBOX, is_k ? &kmap : &vmap, bar, j * 64, row);
   };
+  // the copying warps' lanes hold the pages of 32 tiles
+  int page = -1;
+  auto page_of = [&](int i) {
+    if (i > 0 && (i & 31) == 0) page = sp_table(a, a.prefix_blocks, a.n_prefix_blocks, t0 + i + lane, BN);
+    return __shfl_sync(0xffffffffu, page, i & 31);
+  };
   const bool early = a.window <= 0;  // the first key tile is known before the rows' positions are
-  if (tid == 0) {
-    if (!a.prefix_ok(P)) nvb::record_error(a.err, nvb::kErrBadArgument);
-    if (early) {
-      for (int i = 0; i < KS && i < t1 - t0; ++i) copy(true, i);
-      for (int i = 0; i < VS && i < t1 - t0; ++i) copy(false, i);
-    }
+  if (early && (warp == 0 || warp == 3)) page = sp_table(a, a.prefix_blocks, a.n_prefix_blocks, t0 + lane, BN);
+  if (warp == 0) {
+    if (lane == 0 && !a.prefix_ok(P)) nvb::record_error(a.err, nvb::kErrBadArgument);
+    if (early)
+      for (int i = 0; i < max(KS, VS) && i < t1 - t0; ++i) {
+        const int pg = page_of(i);
+        if (lane == 0 && i < KS) copy(true, i, pg);
+        if (lane == 0 && i < VS) copy(false, i, pg);
+      }
   }
   // The softmax threads load the query rows, into the swizzled layout that the MMA reads (zeros behind the list), and
   // find the rows' positions.
@@ -252,7 +261,8 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
       for (int k = 0; k < CH; ++k) {
         const int f = row0 + tile * 128 + first + k * STEP;
         v[k] = make_uint4(0, 0, 0, 0);
-        if (f < row0 + rows) v[k] = *reinterpret_cast<const uint4*>(src + (long)(f / G) * a.q_tok + (long)(f % G) * a.q_head);
+        const int2 tg = a.split(f);
+        if (f < row0 + rows) v[k] = *reinterpret_cast<const uint4*>(src + (long)tg.x * a.q_tok + (long)tg.y * a.q_head);
       }
 #pragma unroll
       for (int k = 0; k < CH; ++k)
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
     }
     const int first = row0 + (twice ? 0 : tile * 128) + (warp & 3) * 32;
     if (first < row0 + rows) {
-      pos = warp_row_position(a, first / G, rr / G, P);
+      pos = warp_row_position(a, a.split(first).x, a.split(rr).x, P);
       if (rr >= row0 + rows) pos = -1;
     }
     if (!early) {
@@ -291,22 +301,23 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
   if (warp == 0 || warp == 3) {
     // ---------------------------------------------------------------- copies
     const bool is_k = warp == 0;
-    if (lane == 0) {
-      const int NS = is_k ? KS : VS;
-      uint64_t* full = is_k ? k_full : v_full;
-      uint64_t* freeb = is_k ? k_free : v_free;
-      int i = early ? min(NS, nt) : 0;
-      bool ok = true;
-      for (; i < nt; ++i) {
-        if (i >= NS && !tc_wait(&freeb[i % NS], ((i / NS) & 1) ^ 1, a.err, &abort_flag)) {
-          ok = false;
-          break;
-        }
-        copy(is_k, i);
+    const int NS = is_k ? KS : VS;
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* freeb = is_k ? k_free : v_free;
+    if (!early) page = sp_table(a, a.prefix_blocks, a.n_prefix_blocks, t0 + lane, BN);
+    int i = early ? min(NS, nt) : 0;
+    bool ok = true;
+    for (; i < nt; ++i) {
+      const int pg = page_of(i);
+      if (i >= NS && !__all_sync(0xffffffffu, tc_wait(&freeb[i % NS], ((i / NS) & 1) ^ 1, a.err, &abort_flag))) {
+        ok = false;
+        break;
       }
-      if (!ok)  // bounded drain of copies that may still be landing
-        for (int j = (i > NS ? i - NS : 0); j < i; ++j) tc_wait(&full[j % NS], (j / NS) & 1, nullptr, nullptr);
+      if (lane == 0) copy(is_k, i, pg);
+      __syncwarp();
     }
+    if (!ok && lane == 0)  // bounded drain of copies that may still be landing
+      for (int j = (i > NS ? i - NS : 0); j < i; ++j) tc_wait(&full[j % NS], (j / NS) & 1, nullptr, nullptr);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issue
     // descriptors differ from these in the start address alone (16-byte units in the low bits)
@@ -386,7 +397,7 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int steps = tile == 0 ? steps0 : steps1;
     const bool have = rr < row0 + rows;
-    const int t = rr / G, h = kvh * G + rr % G;
+    const int t = a.split(rr).x, h = kvh * G + a.split(rr).y;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_col = lanes + (uint32_t)tile * BN, o_col = lanes + C::O_COL + (uint32_t)tile * HD;
     const float sl2 = a.scale * kLog2e;
@@ -512,9 +523,9 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int f = rr - lane + k * 8 + (lane >> 2);
-          dst[k] = f < row0 + rows
-                       ? pl.part_o + (((long)(f / G) * a.nq + kvh * G + f % G) * NS + part) * HD + (lane & 3) * 4
-                       : nullptr;
+          const int2 tg = a.split(f);
+          dst[k] = f < row0 + rows ? pl.part_o + (((long)tg.x * a.nq + kvh * G + tg.y) * NS + part) * HD + (lane & 3) * 4
+                                   : nullptr;
         }
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
