@@ -15,6 +15,7 @@
 #include <cmath>
 #include <string>
 #include <tuple>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -466,7 +467,7 @@ constexpr size_t sp_mma_smem() {
 // Grid: the parts of the prefix (split fastest, then KV head, then row tile), then those of the sequences' own keys
 // (split, KV head, row tile, sequence).  K/V tiles of 64 keys come through TMA into a ring of STAGES; bound by the
 // bytes of the cache as long as a tile serves few rows.
-template <int HD, int STAGES>
+template <int HD, int STAGES, int MAX_RG>
 __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUtensorMap& vmap, const SpArgs& a,
                                             const SpPlan& pl) {
   extern __shared__ uint8_t smem_raw[];
@@ -563,13 +564,16 @@ __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUten
     }
     return;
   }
-  if (p.rows <= 16) sp_part_mma<HD, STAGES, 1>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
-  else if (p.rows <= 32) sp_part_mma<HD, STAGES, 2>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
-  else sp_part_mma<HD, STAGES, 4>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
+  if (MAX_RG == 1 || p.rows <= 16) sp_part_mma<HD, STAGES, 1>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
+  else if (MAX_RG == 2 || p.rows <= 32)
+    sp_part_mma<HD, STAGES, MAX_RG == 1 ? 1 : 2>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
+  else sp_part_mma<HD, STAGES, MAX_RG>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
 }
 
-template <int HD, int STAGES>
-__global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUtensorMap kmap,
+// ``MAX_RG``: row groups of the largest part.  A CTA spends some 3 us on either side of its stream of tiles, which the
+// others of its SM fill: three of them where the registers allow it (parts of up to 32 rows, head dim up to 128).
+template <int HD, int STAGES, int MAX_RG>
+__global__ void __launch_bounds__(128, HD <= 128 && MAX_RG <= 2 ? 3 : 1) sp_mma_kernel(const __grid_constant__ CUtensorMap kmap,
                                                      const __grid_constant__ CUtensorMap vmap, const SpArgs a,
                                                      const SpPlan pl) {
   // After the tcgen05 kernel nothing here depends on its results: the parts run beside it, on the SMs that it leaves
@@ -577,7 +581,7 @@ __global__ void __launch_bounds__(128) sp_mma_kernel(const __grid_constant__ CUt
   // the end, so that the join, which waits for this kernel, comes after both.
   if (!pl.tc) nvb::pdl_wait();
   nvb::pdl_trigger();
-  sp_mma_part<HD, STAGES>(kmap, vmap, a, pl);
+  sp_mma_part<HD, STAGES, MAX_RG>(kmap, vmap, a, pl);
   if (pl.tc && blockIdx.x == gridDim.x - 1) nvb::pdl_wait();
 }
 
@@ -642,13 +646,13 @@ __global__ void __launch_bounds__(128) sp_join_kernel(SpArgs a, SpPlan pl) {
 
 #include "shared_prefix_tc.cuh"
 
-template <int HD, int STAGES>
+template <int HD, int STAGES, int MAX_RG>
 int launch_split(const SpArgs& a, const SpPlan& pl, const void* kc, const void* vc, cudaStream_t stream) {
   int launches = 1;
   const uint64_t rows = (uint64_t)a.num_blocks * a.nkv * a.block_size;
   const CUtensorMap km = nvb::make_tmap_2d_bf16(kc, rows, HD, HD, KT);
   const CUtensorMap vm = nvb::make_tmap_2d_bf16(vc, rows, HD, HD, KT);
-  auto kern = sp_mma_kernel<HD, STAGES>;
+  auto kern = sp_mma_kernel<HD, STAGES, MAX_RG>;
   constexpr size_t sm = sp_mma_smem<HD, STAGES>();
   C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
   if constexpr (HD <= 128) {
@@ -676,9 +680,10 @@ void split_keys(long groups, int tiles, long ctas, int* n, int* per) {
 // How many splits the tcgen05 kernel takes of the prefix.  Its CTAs have an SM each to themselves and the own keys' kernel
 // runs on the others meanwhile, so the rule looks for the least time of the two together: a prefix CTA takes some 8 us and
 // 1.7 us for every key tile (two tiles when both its row tiles are the same rows); the own keys stream at 6 TB/s, which
-// two thirds of the SMs still reach.  (Measured with 32 and with 148 prefix CTAs: 32 sequences on 2048 keys 24 against
-// 34 us, 128 on 8192 keys 90 against 100 us, 96 on 16000 keys, narrow heads, 241 against 65 us.)
-void split_prefix(int groups, int tiles, bool twice, double own_bytes, int sms, int* n, int* per) {
+// two thirds of the SMs still reach; a split's parts are written and read again at some 2 TB/s.  (Measured with 1, 2, 3, 4,
+// 6, 9 splits: 32 sequences on 2048 keys 33, 26, 25, 24, 26, 29 us; 128 on 8192 keys 152, 90, 84, 88, 92, 98 us; 64 with
+// drafts on 4096 keys 85, 54, 50, 52, 57, 63 us.)
+void split_prefix(int groups, int tiles, bool twice, double own_bytes, double part_bytes, int sms, int* n, int* per) {
   const double own_us = own_bytes / 6.0e6;
   double best = 1e30;
   for (int splits = 1; splits <= tiles && (splits == 1 || (long)splits * groups <= sms); ++splits) {
@@ -686,8 +691,8 @@ void split_prefix(int groups, int tiles, bool twice, double own_bytes, int sms, 
     const double waves = std::ceil((double)splits * groups / sms);
     const double tc = waves * (8.0 + 1.7 * (twice ? (each + 1) / 2 : each));
     const double share = std::min(1.0, 1.5 * std::max(0, sms - splits * groups) / sms);  // of the stream, meanwhile
-    const double total = own_us <= share * tc ? tc : tc + (own_us - share * tc);
-    if (total < best - 0.5) {  // parts are written and read again: more of them only where it shows
+    const double total = (own_us <= share * tc ? tc : tc + (own_us - share * tc)) + splits * part_bytes / 2.0e6;
+    if (total < best) {
       best = total;
       *n = splits;
       *per = each;
@@ -806,8 +811,8 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
     pl.pre_row_tiles = (int)((rows + 255) / 256);
     // half of the keys that the bound leaves to the sequences, on average
     const double own_bytes = 2.0 * (double)(max_len - pre_keys) * (double)(B * nkv * hd);
-    split_prefix((int)(nkv * pl.pre_row_tiles), (int)((pre_keys + 127) / 128), rows <= 128, own_bytes, sms, &pl.n_pre,
-                 &pl.pre_tiles);
+    split_prefix((int)(nkv * pl.pre_row_tiles), (int)((pre_keys + 127) / 128), rows <= 128, own_bytes,
+                 8.0 * (double)(T * nq * hd) * (rows <= 128 ? 2 : 1), sms, &pl.n_pre, &pl.pre_tiles);
     pl.pre_slots = 2 * pl.n_pre;
   } else {
     pl.pre_row_tiles = (int)((rows + kRows - 1) / kRows);
@@ -821,8 +826,18 @@ std::tuple<at::Tensor, int64_t> shared_prefix_attention_cuda(
   pl.part_o = scratch.data_ptr<float>();
   pl.part_lse = pl.part_o + parts * hd;
   const void *kp = k_cache.data_ptr(), *vp = v_cache.data_ptr();
-  const int launches = hd == 64    ? launch_split<64, 4>(a, pl, kp, vp, stream)
-                       : hd == 128 ? launch_split<128, 3>(a, pl, kp, vp, stream)
-                                   : launch_split<256, 2>(a, pl, kp, vp, stream);
+  // rows of the largest part, and K/V in flight: 64 KB a CTA where three share an SM, 96 KB else
+  const int64_t part_rows = std::max<int64_t>(std::min<int64_t>(max_q, T) * G, pl.tc ? 0 : rows);
+  auto launch = [&](auto hd_, auto few, auto many) {
+    constexpr int HD = decltype(hd_)::value, FEW = decltype(few)::value, MANY = decltype(many)::value;
+    return part_rows <= 16   ? launch_split<HD, FEW, 1>(a, pl, kp, vp, stream)
+           : part_rows <= 32 ? launch_split<HD, FEW, 2>(a, pl, kp, vp, stream)
+                             : launch_split<HD, MANY, 4>(a, pl, kp, vp, stream);
+  };
+#define SP_INT(N) std::integral_constant<int, N>()
+  const int launches = hd == 64    ? launch(SP_INT(64), SP_INT(4), SP_INT(4))
+                       : hd == 128 ? launch(SP_INT(128), SP_INT(2), SP_INT(3))
+                                   : launch(SP_INT(256), SP_INT(2), SP_INT(2));
+#undef SP_INT
   return {out, launches};
 }
