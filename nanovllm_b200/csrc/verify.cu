@@ -53,6 +53,10 @@ struct VerifyArgs {
   unsigned long long* cut;
   float* row_max;
   int* accept;
+  // the kept set where it is a list of at most kList tokens: their number (else 0), tokens in order, weights
+  int* kept_n;
+  int* kept_tok;
+  double* kept_w;
   int* err;
 
   NV_DEVICE double uniform(int r) const {
@@ -79,19 +83,20 @@ NV_DEVICE unsigned long long rank_key(float x, int i) {
   return ((unsigned long long)order_key(fmaxf(x, -INFINITY) + 0.f) << 32) | (0xffffffffu - (uint32_t)i);
 }
 
-// 2^(d c) in 64 bits (relative error below 1e-12) for an exponent in [-1000, 0]: it is k / 256 + r, with a table of
-// 2^(k / 256) and three terms of the exponential series for 2^r, |r| <= 1/512 (the fourth is 1.4e-13).
-constexpr int kTable = 256;
+// 2^(d c) in 64 bits (relative error below 1e-12) for an exponent in [-1000, 0]: it is k / 128 + r, with a table of
+// 2^(k / 128) and the exponential series for 2^r, |r| <= R = 1/256, whose fourth term a r^4 is taken as a (R^2 r^2 - R^4 / 8)
+// (off by at most a R^4 / 8 = 2.8e-13).
+constexpr int kTable = 128;
 NV_DEVICE double exp2_64(double d, double c, const double* table) {
-  const double magic = 26388279066624.0;  // 1.5 * 2^44: the last bit of a sum with it is 1/256
+  const double magic = 52776558133248.0;  // 1.5 * 2^45: the last bit of a sum with it is 1/128
   const double t = fma(d, c, magic);
   const double r = fma(d, c, magic - t);
   const int k = max(__double2loint(t), -1000 * kTable);
   double p = 5.550410866482158e-2;
-  p = fma(p, r, 2.402265069591007e-1);
+  p = fma(p, r, 2.402265069591007e-1 + 9.618129107628477e-3 / 65536);
   p = fma(p, r, 6.931471805599453e-1);
-  p = fma(p, r, 1.0) * table[k & (kTable - 1)];
-  return __hiloint2double(__double2hiint(p) + (k >> 8) * (1 << 20), __double2loint(p));
+  p = fma(p, r, 1.0 - 9.618129107628477e-3 / 65536 / 65536 / 8) * table[k & (kTable - 1)];
+  return __hiloint2double(__double2hiint(p) + (k >> 7) * (1 << 20), __double2loint(p));
 }
 NV_DEVICE void fill_table(double* table) {
   if (threadIdx.x < kTable) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / kTable));
@@ -164,6 +169,15 @@ NV_DEVICE T peer_load(const T* p, uint32_t rank) {  // the same variable of anot
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return *reinterpret_cast<T*>(&v);
   }
+}
+
+NV_DEVICE uint4 peer_load4(const uint32_t* p, uint32_t rank) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(nvb::map_peer(nvb::smem_u32(p), rank))
+               : "memory");
+  return v;
 }
 
 template <typename T>
@@ -339,7 +353,10 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   __shared__ int sh_i[kWarps];
   __shared__ unsigned int n_list, n_gather, eq_sh[2][kMaxCluster * kWarps];
   __shared__ unsigned long long keys[kOwnList], found_sh[2];
-  __shared__ double pool[2 * kList];  // the threads' maxima, then rank 0's list: keys, and weights in order
+  // the threads' maxima, then rank 0's list (keys, and weights in order), then a histogram
+  __shared__ __align__(16) double pool[2 * kList];
+  __shared__ double hit_mass;
+  __shared__ int hit_bin, hit_count;
   float* maxima = reinterpret_cast<float*>(pool);
   const int r = blockIdx.x / cluster_size(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
@@ -388,6 +405,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   const bool cut_k = k > 0 && k < V, cut_p = top < 1.f;
   unsigned long long cut = 0;
   double Z = 0.0;
+  int kept_n = 0;  // rank 0: tokens listed for the draw
   float m;
   if (!cut_k && !cut_p && a.softcap <= 0.f) {
     // ---------------------------------------------------------------- no cut: sums against the CTA's own maximum
@@ -445,6 +463,11 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
     cluster_reduce<1, true>(best, red, turn);
     cut = m == -INFINITY ? 0 : best[0];
     Z = 1.0;
+    kept_n = cut != 0;
+    if (rank == 0 && tid == 0 && kept_n != 0) {
+      a.kept_tok[(long)r * kList] = (int)(0xffffffffu - (uint32_t)cut);
+      a.kept_w[(long)r * kList] = 1.0;
+    }
   } else if (cut_k || cut_p || a.softcap > 0.f) {
     const bool cuts = (cut_k || cut_p) && m != -INFINITY;
     // With a cut: this CTA's tokens at or above its threshold, the want_top-th largest of its threads' maxima, so at least
@@ -578,6 +601,17 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         if (!enough || last < 0) return false;
         cut = list[last];
         Z = z;
+        if (count == 0.0) {  // nothing is kept but what is listed: the list in token order
+          kept_n = last + 1;
+          if (tid < kept_n) {
+            const uint32_t low = (uint32_t)list[tid];
+            int at = 0;
+#pragma unroll 4
+            for (int j = 0; j < kept_n; ++j) at += (uint32_t)list[j] > low;
+            a.kept_tok[(long)r * kList + at] = (int)(0xffffffffu - low);
+            a.kept_w[(long)r * kList + at] = w;
+          }
+        }
         return true;
       };
       threshold = nvb::warp_max((uint32_t)lane < CL ? peer_load(&threshold_sh, lane) : -INFINITY);
@@ -588,15 +622,91 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
       unsigned long long told[1] = {rank == 0 && done ? 1ull : 0ull};
       cluster_reduce<1, true>(told, red, turn);
       if (told[0] == 0) {
-        // ------------------------------------------------------------ beyond the list: the range of logits that holds the
-        // cut is quartered until few tokens are left in it, or one logit
+        // ------------------------------------------------------------ beyond the list
         // The smallest kept key when 1 or weights are summed in descending order up to ``target``, of the keys >= floor;
-        // leaves the kept mass in Z when weights are summed.
+        // leaves the kept mass in Z when weights are summed.  A histogram over the first 16 bits of the logits gives the
+        // cut's logit (bf16) or a guess of it; from there, or where its bins end above the cut, the range of logits that
+        // holds the cut is quartered until few tokens are left in it, or one logit.
         auto select = [&](bool by_mass, double target, float lo, unsigned long long floor_key, int slot) {
           float hi = INFINITY;  // the cut's logit is in [lo, hi), while not ``open`` in [lo, m]
           bool open = false;
           double over[2] = {0.0, 0.0};  // sum and count from hi on
           double in_lo = kAll;          // count from lo on
+          float one_logit = NAN, guess_lo = NAN, guess_hi = NAN;
+          kept_n = 0;
+          {
+            uint32_t* bins = reinterpret_cast<uint32_t*>(pool);
+            constexpr int kBins = 4 * kThreads;
+            static_assert(sizeof(pool) == kBins * 4);
+            const uint32_t top_key = order_key(m + 0.f) >> 16;
+            reinterpret_cast<uint4*>(bins)[tid] = make_uint4(0, 0, 0, 0);
+            if (tid == 0) hit_bin = -1;
+            __syncthreads();
+            for (int w = tid; w < s.nw; w += kThreads)
+              s.each(w, [&](float v, int) {
+                const uint32_t at = top_key - (order_key(v + 0.f) >> 16);
+                if (v >= lo && at < (uint32_t)kBins) atomicAdd(&bins[at], 1u);
+              });
+            nvb::cluster_sync();
+            uint4 n4 = make_uint4(0, 0, 0, 0);  // every CTA joins all bins, four a thread
+            for (uint32_t q = 0; q < CL; ++q) {
+              const uint4 v = peer_load4(&bins[4 * tid], q);
+              n4.x += v.x, n4.y += v.y, n4.z += v.z, n4.w += v.w;
+            }
+            const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
+            // a bin's one value (bf16), or the middle of it
+            auto bin_logit = [&](int j) {
+              const uint32_t key = top_key - (4 * tid + j);
+              const uint32_t low = sizeof(T) == 4 ? 0x7fffu : key >= 0x8000u ? 0u : 0xffffu;
+              return key_logit((unsigned long long)(key << 16 | low) << 32);
+            };
+            double mass[4], sum = 0.0;
+            int count = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              mass[j] = n[j] == 0 ? 0.0 : by_mass ? n[j] * rs.weight64(bin_logit(j), table) : (double)n[j];
+              sum += mass[j];
+              count += (int)n[j];
+            }
+            double incl = sum;
+            int incl_n = count;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const double v = __shfl_up_sync(0xffffffffu, incl, o);
+              const int c = __shfl_up_sync(0xffffffffu, incl_n, o);
+              if (lane >= o) incl += v, incl_n += c;
+            }
+            if (lane == 31) sh_d[warp] = incl, sh_i[warp] = incl_n;
+            __syncthreads();
+            int first = 0;  // the first warp that reaches the target, and what lies before it
+            double before = 0.0;
+            int before_n = 0;
+            while (first < kWarps && before + sh_d[first] < target) before += sh_d[first], before_n += sh_i[first], ++first;
+            if (warp == first) {
+              const unsigned over_t = __ballot_sync(0xffffffffu, before + incl >= target);
+              if (lane == __ffs(over_t) - 1) {
+                double c = before + (incl - sum);
+                int nc = before_n + incl_n - count, j = 0;
+                while (j < 3 && c + mass[j] < target) c += mass[j], nc += (int)n[j], ++j;
+                hit_bin = 4 * tid + j;
+                hit_mass = c;
+                hit_count = nc;
+              }
+            }
+            __syncthreads();
+            if (hit_bin >= 0) {
+              const uint32_t key = top_key - hit_bin;
+              if (sizeof(T) == 2) {
+                one_logit = key_logit((unsigned long long)(key << 16 | (key >= 0x8000u ? 0u : 0xffffu)) << 32);
+                over[0] = by_mass ? hit_mass : (double)hit_count;
+                over[1] = (double)hit_count;
+              } else {
+                auto flush = [](float v) { return fabsf(v) < FLT_MIN ? 0.f : v; };
+                guess_lo = fmaxf(lo, flush(key_logit((unsigned long long)(key << 16) << 32)));
+                guess_hi = flush(key_logit((unsigned long long)((key + 1) << 16) << 32));
+              }
+            }
+          }
           // sums and counts of the logits at or above each of three
           auto sums = [&](const float (&t)[3], double (&out)[6]) {
             float acc[3] = {0.f, 0.f, 0.f};
@@ -636,8 +746,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
             return fabsf(n) < FLT_MIN ? 0.f : n;
           };
           const float eps = sizeof(T) == 2 ? 0.00390625f : 1.1920929e-7f;  // half a step, a step of the type
-          float one_logit = NAN;
-          for (int step = 0; step < 300; ++step) {
+          for (int step = 0; step < 300 && isnan(one_logit); ++step) {
             const bool few = in_lo - over[1] <= (double)kList;
             const float top_v = open ? hi : m;
             const bool narrow = top_v - lo <= eps * fmaxf(fabsf(top_v), fabsf(lo)) || step % 8 == 7;
@@ -666,7 +775,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
 #pragma unroll
               for (int q = 0; q < 3; ++q) t[q] = key_logit((unsigned long long)(kl + (q + 1) * part) << 32);
             }
-            if (!(t[0] > lo)) t[0] = t[1] = t[2] = next_up(lo);
+            if (step == 0 && guess_hi > guess_lo) t[0] = guess_lo, t[1] = t[2] = guess_hi;
+            else if (!(t[0] > lo)) t[0] = t[1] = t[2] = next_up(lo);
             double f[6];
             sums(t, f);
             if (f[2] >= target) lo = t[2], in_lo = f[5];
@@ -700,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
           }
           // many equal logits: the n_keep lowest tokens among them, by counts of consecutive words, in token order
           const float v_cut = one_logit;
-          const double one = by_mass ? (double)rs.weight(v_cut) : 1.0;
+          const double one = by_mass ? rs.weight64(v_cut, table) : 1.0;
           const double missing = ceil((target - over[0]) / fmax(one, 1e-300));
           const int n_keep = (int)fmin(fmax(missing, 1.0), 2.0 * kMaxVocab);
           const int per = (s.nw + kWarps - 1) / kWarps, w0 = min(s.nw, warp * per), w1 = min(s.nw, w0 + per);
@@ -770,6 +880,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   if (tid == 0) {
     a.cut[r] = cut;
     a.row_max[r] = m;
+    a.kept_n[r] = kept_n;
   }
   if (drafted) {
     const double w = d >= 0 && rank_key(d_logit, (int)d) >= cut ? rs.weight64(d_logit, table) : 0.0;
@@ -801,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   __shared__ uint64_t bar;
   __shared__ Tables red;
   __shared__ double table[kTable], all_sh[2][kMaxCluster * kWarps + 1], sub_sh[kWarps];
-  __shared__ int sh_i[kWarps];
+  __shared__ int sh_i[kWarps], first_sh[kWarps], last_sh[kWarps];
   const int b = blockIdx.x / cluster_size(), tid = threadIdx.x, V = a.V, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
   const int2 rows = seq_rows(a, b);
@@ -817,7 +928,6 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
     }
     return;
   }
-  cluster_arrive();
   int acc = n - 1;  // accepted drafts: up to the first refusal
   for (int j0 = 0; j0 < n - 1; j0 += 32) {
     const bool no = j0 + lane < n - 1 && !a.accept[rows.x + j0 + lane];
@@ -829,12 +939,76 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   }
   const int r = rows.x + acc;
   const bool rejected = acc < n - 1;
+  auto finish = [&] {
+    for (int j = tid; j < a.max_q; j += kThreads)
+      if (j != acc) out[j] = j < acc ? a.ids[rows.x + j + 1] : -1;
+    if (tid == 0) a.counts[b] = acc + 1;
+  };
+  const int kept_n = a.kept_n[r];
+  if (kept_n > 0) {
+    // ---------------------------------------------------------------- the kept tokens are listed: one CTA, a token a thread
+    if (rank != 0) return;
+    const bool here = tid < kept_n;
+    const int tok = here ? a.kept_tok[(long)r * kList + tid] : 0;
+    const double w = here ? a.kept_w[(long)r * kList + tid] : 0.0;
+    double l = w;
+    // inclusive sums over the CTA; the total in ``total``
+    double total = 0.0;
+    auto scan = [&](double v) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+      }
+      __syncthreads();
+      if (lane == 31) sub_sh[warp] = v;
+      __syncthreads();
+      double base = 0.0;
+      total = 0.0;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < warp) base += sub_sh[i];
+        total += sub_sh[i];
+      }
+      return base + v;
+    };
+    if (rejected) {
+      if (a.probs != nullptr) {
+        const int dr = draft_row(a, b, r, sh_i);
+        scan(w);
+        if (dr < a.D && here) l = fmax(0.0, w * (1.0 / total) - (double)a.probs[dr * a.probs_ld + tok]);
+      } else if (here && a.ids[r + 1] == tok) {
+        l = 0.0;
+      }
+    }
+    double incl = scan(l);
+    if (!(total > 0.0)) {  // nothing is left of p - q: the probabilities themselves
+      l = w;
+      incl = scan(l);
+    }
+    const double want = fmin(fmax(a.uniform(rows.y - 1), 0.0), 1.0 - 2.220446049250313e-16) * total;
+    // the first token whose sum exceeds ``want``; sums that end a rounding before it: the last token with weight
+    const unsigned over = __ballot_sync(0xffffffffu, l > 0.0 && incl > want);
+    const unsigned some = __ballot_sync(0xffffffffu, l > 0.0);
+    if (lane == 0) {
+      first_sh[warp] = over != 0 ? warp * 32 + __ffs(over) - 1 : kThreads;
+      last_sh[warp] = some != 0 ? warp * 32 + 31 - __clz(some) : 0;
+    }
+    __syncthreads();
+    int pick = kThreads, last = 0;
+    for (int i = 0; i < kWarps; ++i) pick = min(pick, first_sh[i]), last = max(last, last_sh[i]);
+    if (tid == (pick < kThreads ? pick : last)) out[acc] = tok;
+    finish();
+    return;
+  }
+  cluster_arrive();
   const Slice<T> s = load_slice(reinterpret_cast<const T*>(a.logits) + r * a.ld, V, buf, &bar);
   const unsigned long long cut = a.cut[r];
   const RowScale rs(a.row_max[r], a.softcap, a.temps[b]);
   const int dr = rejected && a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
   const float* q = rejected && a.probs != nullptr && dr < a.D ? a.probs + dr * a.probs_ld : nullptr;
   const long drafted = rejected && a.probs == nullptr ? a.ids[r + 1] : -1;
+  if (q != nullptr)  // p is summed before q is read: q comes nearer meanwhile
+    for (int i = s.lo + tid * 32; i < s.hi; i += kThreads * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
   fill_table(table);
   finish_slice(s, &bar, a.err);
   cluster_wait();
@@ -995,11 +1169,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
     }
     if (plain == 1 && rank == 0 && tid == 0) out[acc] = 0;  // no logit above -inf
   }
-  if (rank == 0) {
-    for (int j = tid; j < a.max_q; j += kThreads)
-      if (j != acc) out[j] = j < acc ? a.ids[rows.x + j + 1] : -1;
-    if (tid == 0) a.counts[b] = acc + 1;
-  }
+  if (rank == 0) finish();
 }
 
 }  // namespace
@@ -1038,7 +1208,8 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   auto tokens = at::empty({B, max_q}, ids.options());
   auto counts = at::empty({B}, cu_q.options());
   if (B == 0) return {tokens, counts, 0};
-  auto scratch = at::empty({R * 2}, ids.options());  // cut, then largest logit and acceptance
+  // per row: cut; largest logit, acceptance; weights, tokens and number of listed tokens
+  auto scratch = at::empty({R * (2 + kList + kList / 2) + (R + 1) / 2}, ids.options());
   VerifyArgs a{};
   a.logits = logits.data_ptr();
   a.ld = logits.stride(0);
@@ -1061,6 +1232,9 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   a.cut = reinterpret_cast<unsigned long long*>(scratch.data_ptr<int64_t>());
   a.row_max = reinterpret_cast<float*>(scratch.data_ptr<int64_t>() + R);
   a.accept = reinterpret_cast<int*>(a.row_max + R);
+  a.kept_w = reinterpret_cast<double*>(scratch.data_ptr<int64_t>() + 2 * R);
+  a.kept_tok = reinterpret_cast<int*>(a.kept_w + R * kList);
+  a.kept_n = a.kept_tok + R * kList;
   a.err = err.data_ptr<int>();
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool wide = logits.scalar_type() == at::kFloat;
