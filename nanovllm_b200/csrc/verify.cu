@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cfloat>
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -87,11 +88,12 @@ NV_DEVICE unsigned long long rank_key(float x, int i) {
 // 2^(k / 128) and the exponential series for 2^r, |r| <= R = 1/256, whose fourth term a r^4 is taken as a (R^2 r^2 - R^4 / 8)
 // (off by at most a R^4 / 8 = 2.8e-13).
 constexpr int kTable = 128;
+template <bool IN_RANGE = false>  // true: the exponent is known to lie above -1000
 NV_DEVICE double exp2_64(double d, double c, const double* table) {
   const double magic = 52776558133248.0;  // 1.5 * 2^45: the last bit of a sum with it is 1/128
   const double t = fma(d, c, magic);
   const double r = fma(d, c, magic - t);
-  const int k = max(__double2loint(t), -1000 * kTable);
+  const int k = IN_RANGE ? __double2loint(t) : max(__double2loint(t), -1000 * kTable);
   double p = 5.550410866482158e-2;
   p = fma(p, r, 2.402265069591007e-1 + 9.618129107628477e-3 / 65536);
   p = fma(p, r, 6.931471805599453e-1);
@@ -140,8 +142,11 @@ struct RowScale {
   }
   NV_DEVICE float weight(float x) const { return exp2f(log_weight(x)); }
   NV_DEVICE double weight64_simple(float x, const double* table) const {  // no soft-cap, finite m
-    const double w = exp2_64((double)fmaxf(x, floor64) - m64, c64, table);
-    return x >= floor64 ? w : 0.0;  // NaN, -inf: 0
+    return x >= floor64 ? floored64(x, table) : 0.0;  // NaN, -inf: 0
+  }
+  // the same where x >= floor64; else 2^-996 (the floor lies 690 log2(e) < 996 below the largest)
+  NV_DEVICE double floored64(float x, const double* table) const {
+    return exp2_64<true>((double)fmaxf(x, floor64) - m64, c64, table);
   }
   NV_DEVICE double weight64(float x, const double* table) const {
     if (x == m) return m == -INFINITY ? 0.0 : 1.0;
@@ -289,6 +294,24 @@ struct Slice {
   }
 };
 
+// The largest logit of this thread's words (NaN is passed over).
+template <typename T>
+NV_DEVICE float slice_max(const Slice<T>& s) {
+  float m = -INFINITY;
+  if constexpr (sizeof(T) == 2) {  // two at a time
+    __nv_bfloat162 acc = __float2bfloat162_rn(-INFINITY);
+    for (int w = threadIdx.x; w < s.nw; w += kThreads) {
+      const uint4 v = reinterpret_cast<const uint4*>(s.words)[w];
+      const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&v);
+      acc = __hmax2(acc, __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3])));
+    }
+    m = fmaxf(m, fmaxf(__low2float(acc), __high2float(acc)));
+  } else {
+    for (int w = threadIdx.x; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { m = fmaxf(m, v); });
+  }
+  return m;
+}
+
 NV_DEVICE int slice_tokens(int V, int n) { return ((V + n - 1) / n + 7) / 8 * 8; }
 
 // Starts the load; ``finish_slice`` before the words are read.
@@ -357,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   __shared__ __align__(16) double pool[2 * kList];
   __shared__ double hit_mass;
   __shared__ int hit_bin, hit_count;
+  __shared__ unsigned int told;
   float* maxima = reinterpret_cast<float*>(pool);
   const int r = blockIdx.x / cluster_size(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
@@ -400,14 +424,13 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   finish_slice(s, &bar, a.err);
   cluster_wait();
   if (!in_seq) return;  // the whole cluster
-  float mine_max = -INFINITY;
-  for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { mine_max = fmaxf(mine_max, v); });
+  const float mine_max = slice_max(s);
   const bool cut_k = k > 0 && k < V, cut_p = top < 1.f;
   unsigned long long cut = 0;
   double Z = 0.0;
   int kept_n = 0;  // rank 0: tokens listed for the draw
   float m;
-  if (!cut_k && !cut_p && a.softcap <= 0.f) {
+  if (!cut_k && !cut_p && k != 1 && a.softcap <= 0.f) {
     // ---------------------------------------------------------------- no cut: sums against the CTA's own maximum
     const float mw = nvb::warp_max(mine_max);
     if (lane == 0) sh_f[warp] = mw;
@@ -416,7 +439,13 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
     for (int i = 1; i < kWarps; ++i) mc = fmaxf(mc, sh_f[i]);
     const RowScale own(mc, 0.f, temp);
     float z4[4] = {0.f, 0.f, 0.f, 0.f};
-    if (own.simple()) {
+    const float off = -mc * own.c_hi;
+    if (own.simple() && fabsf(off) < 64.f) {  // one product: weights within 1e-5, where near ties are found within 1e-4
+      for (int w = tid; w < s.nw; w += kThreads) {
+        int j = 0;
+        s.each(w, [&](float v, int) { z4[j++ & 3] += exp2f(fmaxf(fmaf(v, own.c_hi, off), -1e30f)); });
+      }
+    } else if (own.simple()) {
       for (int w = tid; w < s.nw; w += kThreads) {
         int j = 0;
         s.each(w, [&](float v, int) { z4[j++ & 3] += exp2f(own.log_weight_simple(v)); });
@@ -424,21 +453,22 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
     } else if (mc == INFINITY) {
       for (int w = tid; w < s.nw; w += kThreads) s.each(w, [&](float v, int) { z4[0] += v == INFINITY ? 1.f : 0.f; });
     }
-    // the CTAs' sums and maxima to every CTA
+    // the CTAs' sums and maxima to rank 0, which alone goes on
     double z = (double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
     if (lane == 0) sh_d[warp] = z;
     __syncthreads();
-    if (tid < (int)CL) {
+    if (tid == 0) {
       z = 0.0;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) z += sh_d[i];
-      peer_store(&red.v[0][0][rank], tid, z);
-      peer_store(&red.v[0][1][rank], tid, (double)mc);
+      peer_store(&red.v[0][0][rank], 0u, z);
+      peer_store(&red.v[0][1][rank], 0u, (double)mc);
     }
-    turn = 1;
-    nvb::cluster_sync();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (rank != 0) return;  // (nobody writes to another CTA than rank 0)
+    cluster_wait();
     const float ml = lane < (int)CL ? (float)red.v[0][1][lane] : -INFINITY;
     const double zl = lane < (int)CL ? red.v[0][0][lane] : 0.0;
     m = nvb::warp_max(ml);
@@ -446,21 +476,20 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
     Z = zl > 0.0 ? zl * all.weight64(ml, table) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) Z += __shfl_xor_sync(0xffffffffu, Z, o);
-  } else {
-    float mv[1] = {mine_max};
-    cluster_reduce<1, true>(mv, red, turn);
-    m = mv[0];
-  }
-  const RowScale rs(m, a.softcap, temp);
-  const bool simple = rs.simple();
-  if (k == 1) {
+  } else if (k == 1) {
     // ---------------------------------------------------------------- greedy: the lowest token among the largest logits
-    unsigned long long best[1] = {0};
-    for (int w = tid; w < s.nw; w += kThreads)
-      s.each(w, [&](float v, int i) {
-        if (v == m && i >= s.lo && i < s.hi) best[0] = max(best[0], rank_key(v, i));
-      });
+    unsigned long long best[1] = {0};  // of each thread's own largest logit
+    for (int w = tid; w < s.nw; w += kThreads) {
+      unsigned same = 0;
+      int j = 0;
+      s.each(w, [&](float v, int) { same |= (v == mine_max ? 1u : 0u) << j++; });
+      for (; same != 0; same &= same - 1) {
+        const int i = s.first + w * Slice<T>::PER + __ffs(same) - 1;
+        if (i >= s.lo && i < s.hi) best[0] = max(best[0], rank_key(mine_max, i));
+      }
+    }
     cluster_reduce<1, true>(best, red, turn);
+    m = best[0] != 0 ? key_logit(best[0]) : -INFINITY;
     cut = m == -INFINITY ? 0 : best[0];
     Z = 1.0;
     kept_n = cut != 0;
@@ -468,12 +497,19 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
       a.kept_tok[(long)r * kList] = (int)(0xffffffffu - (uint32_t)cut);
       a.kept_w[(long)r * kList] = 1.0;
     }
-  } else if (cut_k || cut_p || a.softcap > 0.f) {
+  } else {
+    float mv[1] = {mine_max};
+    cluster_reduce<1, true>(mv, red, turn);
+    m = mv[0];
+  }
+  const RowScale rs(m, a.softcap, temp);
+  const bool simple = rs.simple();
+  if (k != 1 && (cut_k || cut_p || a.softcap > 0.f)) {
     const bool cuts = (cut_k || cut_p) && m != -INFINITY;
     // With a cut: this CTA's tokens at or above its threshold, the want_top-th largest of its threads' maxima, so at least
     // that many; the row's list holds every token at or above the largest threshold of the cluster.  That is enough for a
     // top_k when it holds top_k tokens (two times as many are aimed at), for a top_p when it holds the mass.
-    const int want_top = min(128, (cut_k ? 2 * min(k, kTop) : 160) / (int)CL + 8);
+    const int want_top = min(128, (cut_k ? 2 * min(k, kTop) : 96) / (int)CL + 8);
     if (cuts) {
       maxima[tid] = mine_max;
       __syncthreads();
@@ -487,43 +523,46 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         }
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
-        while (lo < hi) {  // at least want_top threads at lo
+        int n_lo = kThreads;
+        while (lo < hi && n_lo > want_top + want_top / 4) {  // at least want_top threads at lo, a quarter more will do
           const uint32_t mid = lo + (hi - lo) / 2 + 1;
           int n = 0;
 #pragma unroll
           for (int j = 0; j < kThreads / 32; ++j) n += own[j] >= mid;
-          if (__reduce_add_sync(0xffffffffu, n) >= want_top) lo = mid;
+          n = __reduce_add_sync(0xffffffffu, n);
+          if (n >= want_top) lo = mid, n_lo = n;
           else hi = mid - 1;
         }
         if (lane == 0) threshold_sh = key_logit((unsigned long long)lo << 32);
       }
     }
-    float z4[4] = {0.f, 0.f, 0.f, 0.f};
-    if (cuts && cut_k) {
-      // the mass of all tokens is not asked for
-    } else if (simple) {
-      for (int w = tid; w < s.nw; w += kThreads) {
-        int j = 0;
-        s.each(w, [&](float v, int) { z4[j++ & 3] += exp2f(rs.log_weight_simple(v)); });
-      }
-    } else {
-      for (int w = tid; w < s.nw; w += kThreads) {
-        int j = 0;
-        s.each(w, [&](float v, int) { z4[j++ & 3] += rs.weight(v); });
-      }
-    }
-    float threshold = -INFINITY;
+    float threshold = INFINITY;
     if (cuts) {
       __syncthreads();
-      threshold = threshold_sh;
-      for (int w = tid; w < s.nw; w += kThreads)
-        s.each(w, [&](float v, int i) {
-          if (v >= threshold && v > -INFINITY) {
-            const unsigned int at = atomicAdd(&n_list, 1u);
-            if (at < (unsigned int)kOwnList) keys[at] = rank_key(v, i);
-          }
-        });
+      threshold = fmaxf(threshold_sh, -FLT_MAX);
     }
+    float z4[4] = {0.f, 0.f, 0.f, 0.f};
+    // sums the weights and lists what reaches the threshold
+    auto pass = [&](auto weight_of) {
+      for (int w = tid; w < s.nw; w += kThreads) {
+        unsigned listed = 0;
+        int j = 0;
+        s.each(w, [&](float v, int) {
+          z4[j & 3] += weight_of(v);
+          listed |= (v >= threshold ? 1u : 0u) << j;
+          ++j;
+        });
+        if (cuts)
+          for (; listed != 0; listed &= listed - 1) {
+            const int i = w * Slice<T>::PER + __ffs(listed) - 1;
+            const unsigned int at = atomicAdd(&n_list, 1u);
+            if (at < (unsigned int)kOwnList) keys[at] = rank_key(to_float(s.words[i]), s.first + i);
+          }
+      }
+    };
+    if (cuts && cut_k) pass([](float) { return 0.f; });  // the mass of all tokens is not asked for
+    else if (simple) pass([&](float v) { return exp2f(rs.log_weight_simple(v)); });
+    else pass([&](float v) { return rs.weight(v); });
     Z = sum1((double)(z4[0] + z4[1]) + (double)(z4[2] + z4[3]));
     if (cuts) {
       // (the sum was a barrier of the cluster)
@@ -552,13 +591,18 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         __syncthreads();
         const int n = (int)n_gather;
         if (n > kList) return false;
+        if (tid == 0 && (n & 1) != 0) list[n] = 0;  // (two keys are read at a time)
+        __syncthreads();
         // a token's place is the number of larger keys
         static_assert(kList == kThreads);
         const unsigned long long key = tid < n ? list[tid] : 0;
         int place = 0;
         if (tid < n)
 #pragma unroll 4
-          for (int j = 0; j < n; ++j) place += list[j] > key;
+          for (int j = 0; j < (n + 1) / 2; ++j) {
+            const ulonglong2 two = reinterpret_cast<const ulonglong2*>(list)[j];
+            place += (two.x > key) + (two.y > key);
+          }
         __syncthreads();
         if (tid < n) {
           list[place] = key;
@@ -583,24 +627,15 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         if (want < 0.0) want = -want * all;
         const bool keep = tid < n && count + tid < limit && (base + incl - w < want || count + tid == 0.0);
         const int kept = __popc(__ballot_sync(0xffffffffu, keep));  // the kept ones are the first
-        double kw = keep ? w : 0.0;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) kw += __shfl_xor_sync(0xffffffffu, kw, o);
-        __syncthreads();
-        if (lane == 0) {
-          sh_i[warp] = kept;
-          sh_d[warp] = kw;
-        }
+        if (lane == 0) sh_i[warp] = kept;
         __syncthreads();
         int last = -1;
-        double z = mass;
-        for (int i = 0; i < kWarps; ++i) {
-          last += sh_i[i];
-          z += sh_d[i];
-        }
+        for (int i = 0; i < kWarps; ++i) last += sh_i[i];
+        if (tid == last) hit_mass = base + incl;
+        __syncthreads();
         if (!enough || last < 0) return false;
         cut = list[last];
-        Z = z;
+        Z = hit_mass;
         if (count == 0.0) {  // nothing is kept but what is listed: the list in token order
           kept_n = last + 1;
           if (tid < kept_n) {
@@ -619,9 +654,9 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
       if (rank == 0 && (!cut_k || k <= kTop))  // the lists are complete down to the largest threshold
         done = walk(threshold, NAN, 0, 0.0, 0.0, cut_k ? (double)k : kAll,
                     !cut_p ? kAll : cut_k ? -(double)top : (double)top * Z, false);
-      unsigned long long told[1] = {rank == 0 && done ? 1ull : 0ull};
-      cluster_reduce<1, true>(told, red, turn);
-      if (told[0] == 0) {
+      if (rank == 0 && tid < (int)CL) peer_store(&told, tid, done ? 1u : 0u);
+      nvb::cluster_sync();
+      if (told == 0) {
         // ------------------------------------------------------------ beyond the list
         // The smallest kept key when 1 or weights are summed in descending order up to ``target``, of the keys >= floor;
         // leaves the kept mass in Z when weights are summed.  A histogram over the first 16 bits of the logits gives the
@@ -649,9 +684,13 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
               });
             nvb::cluster_sync();
             uint4 n4 = make_uint4(0, 0, 0, 0);  // every CTA joins all bins, four a thread
-            for (uint32_t q = 0; q < CL; ++q) {
-              const uint4 v = peer_load4(&bins[4 * tid], q);
-              n4.x += v.x, n4.y += v.y, n4.z += v.z, n4.w += v.w;
+            for (uint32_t q = 0; q < CL; q += 4) {
+              uint4 v[4];
+#pragma unroll
+              for (uint32_t i = 0; i < 4; ++i)
+                v[i] = q + i < CL ? peer_load4(&bins[4 * tid], q + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) n4.x += v[i].x, n4.y += v[i].y, n4.z += v[i].z, n4.w += v[i].w;
             }
             const uint32_t n[4] = {n4.x, n4.y, n4.z, n4.w};
             // a bin's one value (bf16), or the middle of it
@@ -1015,6 +1054,17 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   const bool simple = cut == 0 && rs.simple();
   const float cut_logit = cut == 0 ? -INFINITY : key_logit(cut);
   constexpr int PER = Slice<T>::PER;
+  const int cut_tok = (int)(0xffffffffu - (uint32_t)cut);
+  // which of a word's tokens are kept, one bit each
+  auto word_kept = [&](int w) {
+    unsigned kept = 0;
+    int j = 0;
+    s.each(w, [&](float v, int i) {
+      kept |= (v >= cut_logit && v > -INFINITY && (v != cut_logit || i <= cut_tok) ? 1u : 0u) << j;
+      ++j;
+    });
+    return kept;
+  };
   // weights of a word's tokens (what a slice's first and last word hold besides weighs nothing); false: nothing
   auto word_weights = [&](int w, double (&l)[PER]) {
     const uint4 raw = reinterpret_cast<const uint4*>(s.words)[w];
@@ -1023,25 +1073,26 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
 #pragma unroll
       for (int j = 0; j < PER; ++j) l[j] = rs.weight64_simple(to_float(e[j]), table);
     } else {
-      bool any = false;  // with a cut most words lie below its logit
+      const unsigned kept = word_kept(w);  // with a cut most words lie below its logit
+      if (kept == 0) return false;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) any |= to_float(e[j]) >= cut_logit;
-      if (!any) return false;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const float v = to_float(e[j]);
-        l[j] = v >= cut_logit && rank_key(v, s.first + w * PER + j) >= cut ? rs.weight64(v, table) : 0.0;
-      }
+      for (int j = 0; j < PER; ++j) l[j] = (kept >> j & 1u) != 0 ? rs.weight64(to_float(e[j]), table) : 0.0;
     }
     return true;
   };
   double Zinv = 1.0;
   if (q != nullptr) {  // p - q needs p itself
-    double z = 0.0, l[PER];
-    for (int w = tid; w < s.nw; w += kThreads) {
-      if (!word_weights(w, l)) continue;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) z += l[j];
+    double z = 0.0;
+    if (simple) {
+      for (int w = tid; w < s.nw; w += kThreads)
+        s.each(w, [&](float v, int) {
+          const double e = rs.floored64(v, table);
+          if (v >= rs.floor64) z += e;
+        });
+    } else {
+      for (int w = tid; w < s.nw; w += kThreads)
+        for (unsigned kept = word_kept(w); kept != 0; kept &= kept - 1)
+          z += rs.weight64(to_float(s.words[w * PER + __ffs(kept) - 1]), table);
     }
     double zs[1] = {z};
     int turn = 0;
@@ -1050,6 +1101,19 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
     Zinv = Z > 0.0 ? 1.0 / Z : 0.0;
   }
   const bool q_aligned = q != nullptr && ((reinterpret_cast<uintptr_t>(q) + 4 * (long)s.first) & 15) == 0;
+  // the draft's probabilities of a word's tokens
+  auto word_q = [&](int i0, float (&qv)[PER]) {
+    if (q_aligned && i0 >= s.lo && i0 + PER <= s.hi) {
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(q + i0 + j);
+        qv[j] = v.x, qv[j + 1] = v.y, qv[j + 2] = v.z, qv[j + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) qv[j] = i0 + j >= s.lo && i0 + j < s.hi ? q[i0 + j] : 0.f;
+    }
+  };
   // what is left of a word's tokens to draw from; plain: the probabilities themselves
   auto word_left = [&](int w, bool plain, double (&l)[PER]) {
     if (!word_weights(w, l)) return false;
@@ -1060,27 +1124,46 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
       for (int j = 0; j < PER; ++j) l[j] = i0 + j == drafted ? 0.0 : l[j];
     } else {
       float qv[PER];
-      if (q_aligned && i0 >= s.lo && i0 + PER <= s.hi) {
+      word_q(i0, qv);
 #pragma unroll
-        for (int j = 0; j < PER; j += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(q + i0 + j);
-          qv[j] = v.x, qv[j + 1] = v.y, qv[j + 2] = v.z, qv[j + 3] = v.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) qv[j] = i0 + j >= s.lo && i0 + j < s.hi ? q[i0 + j] : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < PER; ++j) l[j] = l[j] > 0.0 ? fmax(0.0, l[j] * Zinv - (double)qv[j]) : 0.0;
+      for (int j = 0; j < PER; ++j) l[j] = l[j] > 0.0 ? fmax(0.0, fma(l[j], Zinv, -(double)qv[j])) : 0.0;
     }
     return true;
   };
   auto warp_left = [&](int wa, int wz, bool plain) {  // of words [wa, wz)
     double sum = 0.0, l[PER];
-    for (int w = wa + lane; w < wz; w += 32)
-      if (word_left(w, plain, l))
+    if (simple && (q == nullptr || plain)) {  // the same terms with less to select
+      const int skip = plain || drafted < 0 || drafted >= V ? -1 : (int)drafted;
+      for (int w = wa + lane; w < wz; w += 32)
+        s.each(w, [&](float v, int i) {
+          const double e = rs.floored64(v, table);
+          if (v >= rs.floor64 && i != skip) sum += e;
+        });
+    } else if (simple) {
+      for (int w = wa + lane; w < wz; w += 32) {
+        float qv[PER];
+        word_q(s.first + w * PER, qv);
+        int j = 0;
+        s.each(w, [&](float v, int) {
+          const double left = fma(rs.floored64(v, table), Zinv, -(double)qv[j++]);
+          if (left > 0.0 && v >= rs.floor64) sum += left;
+        });
+      }
+    } else if (cut != 0) {  // a lane takes its kept tokens one by one: they are few
+      for (int w = wa + lane; w < wz; w += 32)
+        for (unsigned kept = word_kept(w); kept != 0; kept &= kept - 1) {
+          const int at = w * PER + __ffs(kept) - 1, i = s.first + at;
+          const double e = rs.weight64(to_float(s.words[at]), table);
+          if (plain) sum += e;
+          else if (q == nullptr) sum += i == drafted ? 0.0 : e;
+          else sum += fmax(0.0, fma(e, Zinv, -(double)q[i]));
+        }
+    } else {
+      for (int w = wa + lane; w < wz; w += 32)
+        if (word_left(w, plain, l))
 #pragma unroll
-        for (int j = 0; j < PER; ++j) sum += l[j];
+          for (int j = 0; j < PER; ++j) sum += l[j];
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
@@ -1240,11 +1323,14 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   const bool wide = logits.scalar_type() == at::kFloat;
   const int64_t width = wide ? 4 : 2;
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // CTAs per row: four of them fit an SM (their slices at most 44 KB), up to 8 while SMs would idle, 16 (beyond the
-  // portable size) for rows that 8 would hold in larger slices
+  // CTAs per row: as few as hold it in slices of 44 KB, four of which fit an SM; 8 while they all run at once (151936
+  // tokens in bf16, 48 rows with a top_p: 50 against 53 us; 577 rows in 8 127, in 7 124 us) and for short rows while SMs
+  // would idle; 16 (beyond the portable size) for rows that 8 would hold in larger slices
   auto cluster_for = [&](int64_t count) {
-    int64_t n = 1;
-    while (n < kMaxCluster && (V * width > n * 44 * 1024 || (n < 8 && count * n * 2 <= sms))) n *= 2;
+    int64_t n = (V * width + 44 * 1024 - 1) / (44 * 1024);
+    if (n > 8) return (int64_t)kMaxCluster;
+    if (n > 3 && count * 8 <= 4 * sms) return (int64_t)8;
+    while (n < 8 && count * n * 2 <= sms) n = std::min<int64_t>(8, n * 2);
     return n;
   };
   auto run = [&](auto kern, int64_t count) {
