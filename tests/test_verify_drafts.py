@@ -339,3 +339,41 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         assert all(torch.equal(o[0], w[0]) and torch.equal(o[1], w[1]) for o, w in zip(outs, want))
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("spread,shift", [(1e-3, 0.0), (3.0, -40.0), (300.0, 0.0), (1e30, 0.0)])
+def test_cuts_far_below_the_largest(spread, shift, dtype, dev):
+    """Cuts beyond any list of the largest, at tiny, negative and huge logits, by count, by mass and by both."""
+    for k, top in ((900, 1.0), (1999, 1.0), (0, 0.9), (0, 0.999999), (1200, 0.97)):
+        s = make([2, 3, 1, 2], 2000, 71, 1.0, k, top, False, dtype, spread=spread)
+        s["logits"] = (s["logits"].float() + shift).to(dtype)
+        s["logits"][0, 17] = s["logits"][0].max() * 4  # one far above: the bins below it start there
+        s["logits"][3] = s["logits"][3].abs().neg()
+        assert call(s, dev) == tuple(oracle(s)), (k, top)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("top", [1.0, 0.9])
+def test_drafts_beyond_32_bits_are_no_token(top, dev):
+    """Such an id is refused, and no token of the vocabulary stands in for it in what is drawn from."""
+    V = 40
+    s = make([2] * 60, V, 73, 1.0, 0, top, spread=0.5)
+    s["ids"][1::2] = s["logits"][::2].argmax(1) + 2 ** 32
+    got = call(s, dev)
+    assert got == tuple(oracle(s)) and all(c == 1 for c in got[1])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("model", [False, True])
+def test_draws_from_short_lists(model, dev):
+    """One to a few hundred kept tokens, refused drafts inside and outside the kept set, nothing left of p - q."""
+    for k, seed in ((1, 81), (2, 82), (31, 83), (64, 84)):
+        s = make([3, 1, 2, 5, 2], 1500, seed, 0.8, k, 0.9, model, torch.bfloat16, good=0.3)
+        assert call(s, dev) == tuple(oracle(s)), k
+    if model:
+        s = make([2, 2, 2], 600, 85, 1.0, 40, 1.0, True, torch.bfloat16)
+        s["draft_probs"][:] = 1.0  # more than p everywhere: the probabilities themselves
+        s["uniforms"][::2] = 0.999
+        assert call(s, dev) == tuple(oracle(s))
