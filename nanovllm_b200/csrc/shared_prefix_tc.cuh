@@ -405,7 +405,21 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
     const bool linear = a.softcap <= 0.f && sl2 > 0.f;  // then the maximum may be taken before the scale
     const float mul = linear ? sl2 : 1.f;
     const bool idle = !have || t >= a.T;  // nothing is written for the row: no need to mask it
+    // O and l scaled by f: at the start of a step the product of the step before is done (its scores came after it)
+    auto rescale_o = [&](float f) {
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        tc_ld32(o_col + c, o);
+        nvb::tmem_ld_wait();
+        nvb::reg_fence<32>(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        tc_st32(o_col + c, o);
+      }
+    };
     float m_used = -INFINITY, l = 0.f;
+    const uint64_t mul2 = pack2(mul, mul);
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
       if (!__all_sync(0xffffffffu, tc_wait(&s_full[tile], (uint32_t)(j & 1), a.err, &abort_flag))) {
@@ -413,90 +427,99 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
         break;
       }
       nvb::tc_fence_after();
-      uint32_t u[BN];
-#pragma unroll
-      for (int c = 0; c < BN; c += 32) tc_ld32(s_col + c, *reinterpret_cast<uint32_t(*)[32]>(u + c));
-      nvb::tmem_ld_wait();
-      nvb::reg_fence<BN>(u);
       const int key0 = (t0 + j * stride + (twice ? tile : 0)) * BN;
-      auto val = [&](int e) { return __uint_as_float(u[e]); };
-      if (!linear) {
-        if (a.softcap > 0.f) {
-#pragma unroll
-          for (int e = 0; e < BN; ++e) u[e] = __float_as_uint(sp_cap(val(e) * a.scale, a.softcap) * kLog2e);
-        } else {
-#pragma unroll
-          for (int e = 0; e < BN; ++e) u[e] = __float_as_uint(val(e) * sl2);
-        }
-      }
       // columns (lo, hi] are seen; a key tile that every row of this warp sees whole skips the masks
       const int hi = min(kend - 1, pos) - key0, lo = pos - win - key0;
-      if (!__all_sync(0xffffffffu, idle || (hi >= BN - 1 && lo < 0))) {
-#pragma unroll
-        for (int e = 0; e < BN; ++e) u[e] = e <= hi && e > lo ? u[e] : 0xff800000u;
-      }
-      // The weights are taken against the maximum in use before this tile's is known: it holds for most tiles, and the
-      // tile's own maximum is found on the way.  Where it does not (or there is none yet), once more.
-      if (!__all_sync(0xffffffffu, m_used > -INFINITY)) {
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int e = 0; e < BN; e += 2) m4[(e >> 1) & 3] = fmaxf(fmaxf(val(e), val(e + 1)), m4[(e >> 1) & 3]);
-        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
-        if (m_used == -INFINITY && mt > -INFINITY) m_used = mt;  // the O row is still zero
-      }
-      const uint64_t mul2 = pack2(mul, mul);
+      const bool whole = __all_sync(0xffffffffu, idle || (hi >= BN - 1 && lo < 0));
+      uint64_t rs0 = 0, rs1 = 0;
+      // 32 columns at a time in a loop, not unrolled: instructions arrive at about one a clock the first time, and the
+      // whole tile unrolled made a CTA's first step take 14000 clocks where the others take 3400.
 #pragma unroll 1
-      for (int again = 0;; ++again) {
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t u[32];
+        tc_ld32(s_col + c, u);
+        nvb::tmem_ld_wait();
+        nvb::reg_fence<32>(u);
+        auto val = [&](int e) { return __uint_as_float(u[e]); };
+        if (!linear) {
+          if (a.softcap > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(sp_cap(val(e) * a.scale, a.softcap) * kLog2e);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(val(e) * sl2);
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) u[e] = c + e <= hi && c + e > lo ? u[e] : 0xff800000u;
+        }
+        // The weights are taken against the maximum in use before these columns' is known: it holds for most of them, and
+        // theirs is found on the way.  Only where there is none yet it is taken first.
+        if (!__all_sync(0xffffffffu, m_used > -INFINITY)) {
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) m4[(e >> 1) & 3] = fmaxf(fmaxf(val(e), val(e + 1)), m4[(e >> 1) & 3]);
+          const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * mul;
+          if (m_used == -INFINITY && mt > -INFINITY) m_used = mt;  // O and the weights before are still zero
+        }
         const float mneg = m_used == -INFINITY ? 0.f : -m_used;  // without keys every score is -inf, every weight 0
         const uint64_t neg2 = pack2(mneg, mneg);
-        uint64_t rs0 = 0, rs1 = 0;
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t w[16];
+        uint64_t sum0 = 0, sum1 = 0;
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t w[16];
+        for (int e = 0; e < 32; e += 2) {
+          const uint64_t v = fma2(pack2(val(e), val(e + 1)), mul2, neg2);
+          const int pair = (e / 2) % 8;
+          float p0, p1;
+          unpack2(v, p0, p1);
+          top4[pair & 3] = fmaxf(fmaxf(p0, p1), top4[pair & 3]);
+          if (pair == 1 || pair == 4 || pair == 6) {
+            exp2_poly2(v, p0, p1);
+          } else {
+            p0 = exp2f(p0);
+            p1 = exp2f(p1);
+          }
+          if (pair & 1) sum1 = add2(sum1, pack2(p0, p1));
+          else sum0 = add2(sum0, pack2(p0, p1));
+          w[e / 2] = nvb::pack_bf16x2(p0, p1);
+        }
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        if (__any_sync(0xffffffffu, top > 8.f)) {
+          // The maximum in use moves; O, l, the weights of the columns before and these ones follow.
+          const float f = top > 8.f ? exp2f(-top) : 1.f;
+          if (top > 8.f) m_used += top;
+          if (j > 0) rescale_o(f);
+          l *= f;
+          rs0 = fma2(rs0, pack2(f, f), 0), rs1 = fma2(rs1, pack2(f, f), 0);
+          tc_st_wait();
+#pragma unroll 1
+          for (int d = 0; d < c; d += 32) {
+            uint32_t q[16];
+            nvb::tmem_ld_32x32b_x16(s_col + d / 2, q);
+            nvb::tmem_ld_wait();
+            nvb::reg_fence<16>(q);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              q[e] = nvb::pack_bf16x2(__uint_as_float(q[e] << 16) * f, __uint_as_float(q[e] & 0xffff0000u) * f);
+            tc_st16(s_col + d / 2, q);
+          }
+          const float now = m_used == -INFINITY ? 0.f : -m_used;
+          sum0 = sum1 = 0;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const uint64_t v = fma2(pack2(val(c + e), val(c + e + 1)), mul2, neg2);
-            const int pair = (e / 2) % 8;
-            float p0, p1;
-            unpack2(v, p0, p1);
-            m4[pair & 3] = fmaxf(fmaxf(p0, p1), m4[pair & 3]);
-            if (pair == 1 || pair == 4 || pair == 6) {
-              exp2_poly2(v, p0, p1);
-            } else {
-              p0 = exp2f(p0);
-              p1 = exp2f(p1);
-            }
-            if (pair & 1) rs1 = add2(rs1, pack2(p0, p1));
-            else rs0 = add2(rs0, pack2(p0, p1));
+            const float p0 = exp2f(fmaf(val(e), mul, now)), p1 = exp2f(fmaf(val(e + 1), mul, now));
+            sum0 = add2(sum0, pack2(p0, p1));
             w[e / 2] = nvb::pack_bf16x2(p0, p1);
           }
-          tc_st16(s_col + c / 2, w);  // over the scores, which are in registers
         }
-        const float over = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));  // how far above the maximum in use
-        if (again > 0 || !__any_sync(0xffffffffu, over > 8.f)) {
-          float r0, r1;
-          unpack2(add2(rs0, rs1), r0, r1);
-          l += r0 + r1;
-          break;
-        }
-        // m_used moves: O and l follow.  Scores of this tile are there, so the product of the step before is done.
-        const float f = over > 8.f ? exp2f(-over) : 1.f;
-        if (over > 8.f) m_used += over;
-        l *= f;
-        if (j > 0) {
-#pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t o[32];
-            tc_ld32(o_col + c, o);
-            nvb::tmem_ld_wait();
-            nvb::reg_fence<32>(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tc_st32(o_col + c, o);
-          }
-        }
+        rs0 = add2(rs0, sum0), rs1 = add2(rs1, sum1);
+        tc_st16(s_col + c / 2, w);  // over scores that have been read
       }
+      float r0, r1;
+      unpack2(add2(rs0, rs1), r0, r1);
+      l += r0 + r1;
       tc_st_wait();
       nvb::tc_fence_before();
       __syncwarp();
@@ -507,46 +530,39 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
     if (ok && steps > 0 && lane == 0) okw = tc_wait(&o_done[tile], (uint32_t)((steps - 1) & 1), a.err, &abort_flag) ? 1 : 0;
     okw = __shfl_sync(0xffffffffu, okw, 0);
     nvb::tc_fence_after();
-    if (okw) {
+    asm volatile("bar.sync 2, 256;" ::: "memory");  // both tiles' products are done: the rings are free
+    if (okw && *reinterpret_cast<volatile int*>(&abort_flag) == 0 && have) {
       const int NS = pl.slots(), part = 2 * split + (twice ? tile : 0);
+      const long slot = ((long)t * a.nq + h) * NS + part;
+      pl.part_lse[slot] = l > 0.f ? m_used + log2f(l) : -INFINITY;
+      if (!twice) pl.part_lse[slot + 1] = -INFINITY;
+    }
+    if (okw && *reinterpret_cast<volatile int*>(&abort_flag) == 0 && steps > 0) {
+      // Each thread lays its row of O into shared memory (rows 16 bytes more than their length apart: no bank conflicts)
+      // and copies it out as a whole: stores of 64 bytes a row took 9000 clocks for 256 rows, these a third of it.
+      constexpr int PITCH = HD * 4 + 16;
+      static_assert(256 * PITCH <= (KS + VS) * C::KTILE, "rows of O in the rings");
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      if (have) {
-        const long slot = ((long)t * a.nq + h) * NS + part;
-        pl.part_lse[slot] = l > 0.f ? m_used + log2f(l) : -INFINITY;
-        if (!twice) pl.part_lse[slot + 1] = -INFINITY;
-      }
-      if (steps > 0) {
-        // 16 columns at a time through shared memory, so that four lanes write 64 consecutive bytes of a row.  The space
-        // is this tile's Q (its products are done), with one set of rows the second Q tile, which is not used.
-        uint8_t* st = qs + (twice ? C::QTILE + (warp - 4) * 2048 : tile * C::QTILE + (warp & 3) * 2048);
-        float* dst[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int f = rr - lane + k * 8 + (lane >> 2);
-          const int2 tg = a.split(f);
-          dst[k] = f < row0 + rows ? pl.part_o + (((long)tg.x * a.nq + kvh * G + tg.y) * NS + part) * HD + (lane & 3) * 4
-                                   : nullptr;
-        }
+      uint8_t* st = kring + (tile * 128 + r) * PITCH;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
-          uint32_t u[16];
-          nvb::tmem_ld_32x32b_x16(o_col + c, u);
-          nvb::tmem_ld_wait();
-          nvb::reg_fence<16>(u);
-          __syncwarp();
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        tc_ld32(o_col + c, o);
+        nvb::tmem_ld_wait();
+        nvb::reg_fence<32>(o);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<float4*>(st + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
-                make_float4(__uint_as_float(u[4 * k]) * inv, __uint_as_float(u[4 * k + 1]) * inv,
-                            __uint_as_float(u[4 * k + 2]) * inv, __uint_as_float(u[4 * k + 3]) * inv);
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = k * 8 + (lane >> 2);
-            const float4 v = *reinterpret_cast<const float4*>(st + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
-            if (dst[k] != nullptr) *reinterpret_cast<float4*>(dst[k] + c) = v;
-          }
-        }
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<float4*>(st + c * 4 + k * 16) =
+              make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv,
+                          __uint_as_float(o[4 * k + 2]) * inv, __uint_as_float(o[4 * k + 3]) * inv);
+      }
+      nvb::fence_proxy_async();
+      if (have) {
+        const float* dst = pl.part_o + (((long)t * a.nq + h) * pl.slots() + 2 * split + (twice ? tile : 0)) * HD;
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(nvb::smem_u32(st)),
+                     "r"(HD * 4)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
       }
     }
   }
