@@ -570,6 +570,9 @@ __device__ __forceinline__ void sp_mma_part(const CUtensorMap& kmap, const CUten
   else sp_part_mma<HD, STAGES, MAX_RG>(a, pl, p, &kmap, &vmap, ring, bars, qs, row_pos, &abort_flag);
 }
 
+// The own keys (and the prefix where no tcgen05 kernel takes it) on mma.sync: a part has at most 64 rows, usually the few
+// of one sequence, and reads its keys once, so it is bound by the bytes of K and V.  Measured: 128 sequences of 64 to 1024
+// own keys, 8 KV heads, 285 MB: 56 us (5.1 TB/s), beside the prefix on a third of the SMs 72 us.
 // ``MAX_RG``: row groups of the largest part.  A CTA spends some 3 us on either side of its stream of tiles, which the
 // others of its SM fill: three of them where the registers allow it (parts of up to 32 rows, head dim up to 128).
 template <int HD, int STAGES, int MAX_RG>
@@ -585,7 +588,7 @@ __global__ void __launch_bounds__(128, HD <= 128 && MAX_RG <= 2 ? 3 : 1) sp_mma_
   if (pl.tc && blockIdx.x == gridDim.x - 1) nvb::pdl_wait();
 }
 
-// One warp per (token, head): joins the parts.
+// One warp per (token, head): joins the parts.  Bound by the latency of two dependent reads, 6 to 11 us.
 template <int HD>
 __global__ void __launch_bounds__(128) sp_join_kernel(SpArgs a, SpPlan pl) {
   nvb::pdl_wait();
@@ -678,20 +681,21 @@ void split_keys(long groups, int tiles, long ctas, int* n, int* per) {
 }
 
 // How many splits the tcgen05 kernel takes of the prefix.  Its CTAs have an SM each to themselves and the own keys' kernel
-// runs on the others meanwhile, so the rule looks for the least time of the two together: a prefix CTA takes some 8 us and
+// runs on the others meanwhile, so the rule looks for the least time of the two together: a prefix CTA takes some 5 us and
 // 1.7 us for every key tile (two tiles when both its row tiles are the same rows); the own keys stream at 6 TB/s, which
-// two thirds of the SMs still reach; a split's parts are written and read again at some 2 TB/s.  (Measured with 1, 2, 3, 4,
-// 6, 9 splits: 32 sequences on 2048 keys 33, 26, 25, 24, 26, 29 us; 128 on 8192 keys 152, 90, 84, 88, 92, 98 us; 64 with
-// drafts on 4096 keys 85, 54, 50, 52, 57, 63 us.)
+// two thirds of the SMs still reach; a split's parts are written and read again at some 1.3 TB/s.  (Measured with 1, 2, 3,
+// 4, 5, 6, 8 splits: 32 sequences on 2048 keys 30, 23, 22, 21, 21, 23, 26 us; 128 on 8192 keys 143, 82, 72, 77, 81, 85,
+// 91 us; 64 with drafts on 4096 keys 83, 51, 41, 49, 48, 51, 57 us; 96 on 16000 keys, head dim 64, 238, 127, 90, 73, 61,
+// 61, 67 us.  Taken are 4, 3, 3 and 6.)
 void split_prefix(int groups, int tiles, bool twice, double own_bytes, double part_bytes, int sms, int* n, int* per) {
   const double own_us = own_bytes / 6.0e6;
   double best = 1e30;
   for (int splits = 1; splits <= tiles && (splits == 1 || (long)splits * groups <= sms); ++splits) {
     const int each = (tiles + splits - 1) / splits;
     const double waves = std::ceil((double)splits * groups / sms);
-    const double tc = waves * (8.0 + 1.7 * (twice ? (each + 1) / 2 : each));
+    const double tc = waves * (5.0 + 1.7 * (twice ? (each + 1) / 2 : each));
     const double share = std::min(1.0, 1.5 * std::max(0, sms - splits * groups) / sms);  // of the stream, meanwhile
-    const double total = (own_us <= share * tc ? tc : tc + (own_us - share * tc)) + splits * part_bytes / 2.0e6;
+    const double total = (own_us <= share * tc ? tc : tc + (own_us - share * tc)) + splits * part_bytes / 1.3e6;
     if (total < best) {
       best = total;
       *n = splits;

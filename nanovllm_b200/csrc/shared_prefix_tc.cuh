@@ -4,14 +4,16 @@
 // rows whatever sequence they come from.  One CTA per (range of keys, KV head, 256 rows) works on two tiles at once:
 // while the softmax threads of one turn its scores into weights, the tensor cores run the other's products.
 //   S_q = Q_q K^T    operands in shared memory, fp32 scores in tensor memory (128 columns per tile)
-//   P_q = 2^(S - m)  one thread per row: scores from tensor memory twice (maximum, then weights), P back as bf16 over the
-//                    first half of the scores' columns
+//   P_q = 2^(S - m)  one thread per row: scores from tensor memory, 32 columns at a time, P back as bf16 (rounded once,
+//                    2^-9 of a weight; sums take the 32 bits) over columns that have been read
 //   O_q += P_q V     A = P from tensor memory, B = V in shared memory, fp32 O in tensor memory
 // With more than 128 rows the two tiles are rows [0, 128) and [128, 256) against every key tile; with fewer, both are
 // the same rows, one against the even key tiles of the range, the other against the odd ones, and each writes a part.
 // The maximum in use moves (and O, l are rescaled) only when a row's maximum grows by more than 2^8: weights stay
 // below 2^8 and O / l is exact all the same.  Both products of a tile take as long as its exponentials (head dim 128:
-// 1024 clocks each), so the kernel is bound by either pipe at best.
+// 1024 clocks each), so the kernel is bound by either pipe at best.  Measured: a step of both tiles takes 3400 clocks and
+// a CTA some 5 us beside its steps; 128 rows x 4 heads against 8192 keys 57 us in 48 CTAs of 22 tiles, 32 x 4 against
+// 2048 keys 15 us.
 //
 // Warps: 0 / 3 copy K / V tiles (TMA), 1 issues the MMAs, 2 clears the V rows behind the prefix, 4-7 and 8-11 are the
 // softmax threads of the two tiles.  Every wait is bounded.
