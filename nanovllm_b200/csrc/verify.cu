@@ -359,11 +359,15 @@ NV_DEVICE void finish_slice(const Slice<T>& s, uint64_t* bar, int* err) {
 }
 
 // One cluster per row: the kept set and, where the row holds a draft, its acceptance.  The row stays in the cluster's
-// shared memory, every pass after the load reads it there; bound by the bytes of the logits.
-//   no cut     each CTA's maximum and sum of weights against it, joined by one exchange
-//   top_k 1    maximum, its lowest token
+// shared memory, every pass after the load reads it there.
+//   no cut     each CTA's maximum and sum of weights against it, joined in rank 0 by one exchange
+//   top_k 1    the lowest token of the largest logit, by one exchange
 //   cuts       some hundred of the largest logits are ranked and walked, in one CTA; a cut that lies beyond them (a flat
-//              row, a large top_k) is found by passes that sum what lies above three thresholds each
+//              row, a large top_k) is found by a histogram, where that does not reach it by passes that sum what lies
+//              above three thresholds each
+// Few rows are bound by the chain of these steps (5 rows of 151936 tokens with a top_p: 14 us, of which 3 us each are the
+// load, the pass that sums and lists, and the ranking), many by the issue of instructions (577 rows without a cut: 60 us,
+// 2.9 TB/s of logits, 14 instructions a token with the exponential's).
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyArgs a) {
   nvb::pdl_wait();
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   if (drafted && rank == 0) {
     const int dr = a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
     d = a.ids[r + 1];
-    if (a.probs != nullptr && dr >= a.D) {
+    if (a.probs != nullptr && (dr < 0 || dr >= a.D)) {
       if (tid == 0) nvb::record_error(a.err, nvb::kErrBadArgument);
       d = -1;
     }
@@ -942,7 +946,10 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
 }
 
 // One cluster per sequence: the accepted drafts and the drawn token.  Weights and sums in 64 bits: the token depends on
-// which side of a sum the uniform falls, and a row has as many sums as tokens.
+// which side of a sum the uniform falls, and a row has as many sums as tokens.  Where the kept tokens are listed one CTA
+// draws from the list (6 us for any batch that fits the GPU at once); else the row is summed, once for p and once more
+// for p - q: 128 rows of 151936 tokens with drafters' distributions 70 us, bound by the issue of some 25 instructions a
+// token and pass.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyArgs a) {
   nvb::pdl_wait();
@@ -987,8 +994,9 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   if (kept_n > 0) {
     // ---------------------------------------------------------------- the kept tokens are listed: one CTA, a token a thread
     if (rank != 0) return;
-    const bool here = tid < kept_n;
+    bool here = tid < kept_n;
     const int tok = here ? a.kept_tok[(long)r * kList + tid] : 0;
+    here = here && tok >= 0 && tok < V;  // (a row that no sequence of a malformed cu_q holds has no list)
     const double w = here ? a.kept_w[(long)r * kList + tid] : 0.0;
     double l = w;
     // inclusive sums over the CTA; the total in ``total``
@@ -1014,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
       if (a.probs != nullptr) {
         const int dr = draft_row(a, b, r, sh_i);
         scan(w);
-        if (dr < a.D && here) l = fmax(0.0, w * (1.0 / total) - (double)a.probs[dr * a.probs_ld + tok]);
+        if (dr >= 0 && dr < a.D && here) l = fmax(0.0, w * (1.0 / total) - (double)a.probs[dr * a.probs_ld + tok]);
       } else if (here && a.ids[r + 1] == tok) {
         l = 0.0;
       }
@@ -1044,7 +1052,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   const unsigned long long cut = a.cut[r];
   const RowScale rs(a.row_max[r], a.softcap, a.temps[b]);
   const int dr = rejected && a.probs != nullptr ? draft_row(a, b, r, sh_i) : 0;
-  const float* q = rejected && a.probs != nullptr && dr < a.D ? a.probs + dr * a.probs_ld : nullptr;
+  const float* q = rejected && a.probs != nullptr && dr >= 0 && dr < a.D ? a.probs + dr * a.probs_ld : nullptr;
   const long drafted = rejected && a.probs == nullptr ? a.ids[r + 1] : -1;
   if (q != nullptr)  // p is summed before q is read: q comes nearer meanwhile
     for (int i = s.lo + tid * 32; i < s.hi; i += kThreads * 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));

@@ -377,3 +377,17 @@ def test_draws_from_short_lists(model, dev):
         s["draft_probs"][:] = 1.0  # more than p everywhere: the probabilities themselves
         s["uniforms"][::2] = 0.999
         assert call(s, dev) == tuple(oracle(s))
+
+
+@gpu
+@pytest.mark.parametrize("cu", [[0, 10, 2, 12], [0, 3, 1, 12], [5, 3, 12, 12], [0, 2, 0, 2, 0, 2]])
+def test_overlapping_sequences_are_reported(cu):
+    """cu_q that falls: the call reports it; what it writes stays inside its outputs."""
+    s = make([3, 4, 5], 900, 91, 0.8, 20, 0.9, True, torch.bfloat16)
+    s["cu_q"], s["max_q"] = torch.tensor(cu, dtype=torch.int32), 12
+    for k in ("temps", "top_ks", "top_ps"):
+        s[k] = s[k][:1].expand(len(cu) - 1).contiguous()
+    with pytest.raises(DeviceWaitTimeout):
+        call(s, "cuda")
+    s = make([3, 4, 5], 900, 91, 0.8, 20, 0.9, True, torch.bfloat16)
+    assert call(s, "cuda") == tuple(oracle(s))
