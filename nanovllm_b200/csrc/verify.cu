@@ -15,6 +15,7 @@
 
 #include <cfloat>
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 #include <tuple>
@@ -1263,6 +1264,19 @@ __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyAr
   if (rank == 0) finish();
 }
 
+// What the largest launch needs, once per device: the same values every time, so calls from several threads may meet here.
+void allow_launches(int device) {
+  static std::atomic<bool> done[64];
+  if (device < 64 && done[device].load()) return;
+  constexpr int kSmem = kMaxVocab * 4 / kMaxCluster + 64;
+  static_assert(kSmem >= 44 * 1024 + 64);
+  for (auto kern : {verify_rows_kernel<float>, verify_rows_kernel<bf16>, verify_draw_kernel<float>, verify_draw_kernel<bf16>}) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  }
+  if (device < 64) done[device].store(true);
+}
+
 }  // namespace
 
 // logits [R, V] bf16 or fp32; ids [R] int64; cu_q [B + 1] int32; temps / topk / topp [B]; uniforms [R] fp32 or fp64;
@@ -1327,6 +1341,7 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   a.kept_tok = reinterpret_cast<int*>(a.kept_w + R * kList);
   a.kept_n = a.kept_tok + R * kList;
   a.err = err.data_ptr<int>();
+  allow_launches(logits.get_device());
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool wide = logits.scalar_type() == at::kFloat;
   const int64_t width = wide ? 4 : 2;
@@ -1344,8 +1359,6 @@ std::tuple<at::Tensor, at::Tensor, int64_t> verify_drafts_cuda(
   auto run = [&](auto kern, int64_t count) {
     const int64_t n = cluster_for(count);
     const size_t smem = (size_t)(((V + n - 1) / n + 7) / 8 * 8 * width + 32);
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (n > 8) C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     C10_CUDA_CHECK(nvb::launch_cluster(kern, dim3((unsigned)(n * count)), dim3(kThreads), smem, stream, (unsigned)n, a));
   };
   if (R > 0) {
