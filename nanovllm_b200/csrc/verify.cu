@@ -576,6 +576,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
       // walked, behind ``count`` tokens of the mass ``mass``.  Kept are the first ``limit`` tokens, while the mass before
       // is below ``want`` (negative: below that share of the mass that the limit leaves).  False when the list is too long
       // or, unless it is ``certain`` to hold the cut, ends before it.
+      bool done = false, tie = false;
       auto walk = [&](float from, float to, unsigned long long floor_key, double count, double mass, double limit,
                       double want, bool certain) {
         unsigned long long* list = reinterpret_cast<unsigned long long*>(pool);
@@ -630,6 +631,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         }
         const bool enough = certain || (limit < kAll ? count + n >= limit : all >= want);
         if (want < 0.0) want = -want * all;
+        else if (!certain)  // a share of Z, whose 32-bit terms leave it up to 4e-6 off
+          tie = __syncthreads_or(tid < n && fabs(base + incl - w - want) <= 4e-6 * want) != 0;
         const bool keep = tid < n && count + tid < limit && (base + incl - w < want || count + tid == 0.0);
         const int kept = __popc(__ballot_sync(0xffffffffu, keep));  // the kept ones are the first
         if (lane == 0) sh_i[warp] = kept;
@@ -655,12 +658,21 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         return true;
       };
       threshold = nvb::warp_max((uint32_t)lane < CL ? peer_load(&threshold_sh, lane) : -INFINITY);
-      bool done = false;
-      if (rank == 0 && (!cut_k || k <= kTop))  // the lists are complete down to the largest threshold
-        done = walk(threshold, NAN, 0, 0.0, 0.0, cut_k ? (double)k : kAll,
-                    !cut_p ? kAll : cut_k ? -(double)top : (double)top * Z, false);
-      if (rank == 0 && tid < (int)CL) peer_store(&told, tid, done ? 1u : 0u);
-      nvb::cluster_sync();
+#pragma unroll 1
+      for (int round = 0;; ++round) {
+        if (rank == 0 && (!cut_k || k <= kTop))  // the lists are complete down to the largest threshold
+          done = walk(threshold, NAN, 0, 0.0, 0.0, cut_k ? (double)k : kAll,
+                      !cut_p ? kAll : cut_k ? -(double)top : (double)top * Z, false);
+        if (rank == 0 && tid < (int)CL) peer_store(&told, tid, round == 0 && tie ? 2u : done ? 1u : 0u);
+        nvb::cluster_sync();
+        if (told != 2) break;
+        // the mass before a token is within that of top Z: once more with Z from 64-bit weights
+        double z = 0.0;
+#pragma unroll 1
+        for (int i = tid; i < s.nw * Slice<T>::PER; i += kThreads) z += rs.weight64(to_float(s.words[i]), table);
+        if (tid == 0) n_gather = 0;
+        Z = sum1(z);
+      }
       if (told == 0) {
         // ------------------------------------------------------------ beyond the list
         // The smallest kept key when 1 or weights are summed in descending order up to ``target``, of the keys >= floor;

@@ -391,3 +391,17 @@ def test_overlapping_sequences_are_reported(cu):
         call(s, "cuda")
     s = make([3, 4, 5], 900, 91, 0.8, 20, 0.9, True, torch.bfloat16)
     assert call(s, "cuda") == tuple(oracle(s))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("equal,top", [(2, 0.5), (4, 0.25), (4, 0.75), (8, 0.5)])
+@pytest.mark.parametrize("gap", [30.0, 24.0, 60.0])
+def test_top_p_at_the_edge_of_equal_logits(gap, equal, top, dev):
+    """Equal largest logits and next to nothing else: top_p falls on the sum of some of them but for that rest, which
+    decides whether one more is kept (gap 60: 1e-23 of the mass, none in 64 bits either)."""
+    g = torch.Generator().manual_seed(97)
+    s = make([1] * 24, 4000, 97, 1.0, 0, top, dtype=torch.bfloat16)
+    x = torch.full((24, 4000), -gap)
+    x.scatter_(1, torch.stack([torch.randperm(4000, generator=g)[:equal] for _ in range(24)]), 0.0)
+    s["logits"] = x.bfloat16()
+    assert call(s, dev) == tuple(oracle(s))
