@@ -368,7 +368,7 @@ NV_DEVICE void finish_slice(const Slice<T>& s, uint64_t* bar, int* err) {
 //              above three thresholds each
 // Few rows are bound by the chain of these steps (5 rows of 151936 tokens with a top_p: 14 us, of which 3 us each are the
 // load, the pass that sums and lists, and the ranking), many by the issue of instructions (577 rows without a cut: 60 us,
-// 2.9 TB/s of logits, 14 instructions a token with the exponential's).
+// 2.9 TB/s of logits, 13 instructions a token with the exponential's).
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyArgs a) {
   nvb::pdl_wait();
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   __shared__ __align__(16) double pool[2 * kList];
   __shared__ double hit_mass;
   __shared__ int hit_bin, hit_count;
-  __shared__ unsigned int told;
+  __shared__ unsigned int told, tie;  // tie: 1 when top_p falls on a sum of the list, 2 once that is resolved
   float* maxima = reinterpret_cast<float*>(pool);
   const int r = blockIdx.x / cluster_size(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const uint32_t rank = nvb::cluster_ctarank(), CL = cluster_size();
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
   }
   fill_table(table);
   if (tid == 0) {
-    n_list = n_gather = 0;
+    n_list = n_gather = tie = 0;
     found_sh[0] = found_sh[1] = 0;
   }
   finish_slice(s, &bar, a.err);
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
       // walked, behind ``count`` tokens of the mass ``mass``.  Kept are the first ``limit`` tokens, while the mass before
       // is below ``want`` (negative: below that share of the mass that the limit leaves).  False when the list is too long
       // or, unless it is ``certain`` to hold the cut, ends before it.
-      bool done = false, tie = false;
+      bool done = false;
       auto walk = [&](float from, float to, unsigned long long floor_key, double count, double mass, double limit,
                       double want, bool certain) {
         unsigned long long* list = reinterpret_cast<unsigned long long*>(pool);
@@ -631,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
         }
         const bool enough = certain || (limit < kAll ? count + n >= limit : all >= want);
         if (want < 0.0) want = -want * all;
-        else if (!certain)  // a share of Z, whose 32-bit terms leave it up to 4e-6 off
-          tie = __syncthreads_or(tid < n && fabs(base + incl - w - want) <= 4e-6 * want) != 0;
+        else if (!certain && tid < n && fabs(base + incl - w - want) <= 4e-6 * want && tie == 0)
+          tie = 1;  // a share of Z, whose 32-bit terms leave it up to 4e-6 off
         const bool keep = tid < n && count + tid < limit && (base + incl - w < want || count + tid == 0.0);
         const int kept = __popc(__ballot_sync(0xffffffffu, keep));  // the kept ones are the first
         if (lane == 0) sh_i[warp] = kept;
@@ -659,18 +659,18 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
       };
       threshold = nvb::warp_max((uint32_t)lane < CL ? peer_load(&threshold_sh, lane) : -INFINITY);
 #pragma unroll 1
-      for (int round = 0;; ++round) {
+      for (;;) {
         if (rank == 0 && (!cut_k || k <= kTop))  // the lists are complete down to the largest threshold
           done = walk(threshold, NAN, 0, 0.0, 0.0, cut_k ? (double)k : kAll,
                       !cut_p ? kAll : cut_k ? -(double)top : (double)top * Z, false);
-        if (rank == 0 && tid < (int)CL) peer_store(&told, tid, round == 0 && tie ? 2u : done ? 1u : 0u);
+        if (rank == 0 && tid < (int)CL) peer_store(&told, tid, tie == 1 ? 2u : done ? 1u : 0u);
         nvb::cluster_sync();
         if (told != 2) break;
         // the mass before a token is within that of top Z: once more with Z from 64-bit weights
         double z = 0.0;
 #pragma unroll 1
         for (int i = tid; i < s.nw * Slice<T>::PER; i += kThreads) z += rs.weight64(to_float(s.words[i]), table);
-        if (tid == 0) n_gather = 0;
+        if (tid == 0) n_gather = 0, tie = 2;
         Z = sum1(z);
       }
       if (told == 0) {
@@ -961,8 +961,8 @@ __global__ void __launch_bounds__(kThreads, 4) verify_rows_kernel(const VerifyAr
 // One cluster per sequence: the accepted drafts and the drawn token.  Weights and sums in 64 bits: the token depends on
 // which side of a sum the uniform falls, and a row has as many sums as tokens.  Where the kept tokens are listed one CTA
 // draws from the list (6 us for any batch that fits the GPU at once); else the row is summed, once for p and once more
-// for p - q: 128 rows of 151936 tokens with drafters' distributions 70 us, bound by the issue of some 25 instructions a
-// token and pass.
+// for p - q: 128 rows of 151936 tokens with drafters' distributions 70 us, bound by the issue of 28 instructions a token
+// and pass.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) verify_draw_kernel(const VerifyArgs a) {
   nvb::pdl_wait();
