@@ -591,18 +591,17 @@ __global__ void __launch_bounds__(128, HD <= 128 && MAX_RG <= 2 ? 3 : 1) sp_mma_
 // One warp per (token, head): joins the parts.  Bound by the latency of two dependent reads, 6 to 11 us.
 template <int HD>
 __global__ void __launch_bounds__(128) sp_join_kernel(SpArgs a, SpPlan pl) {
-  nvb::pdl_wait();
-  nvb::pdl_trigger();
-  const long row = ((long)blockIdx.x * 128 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (row >= (long)a.T * a.nq) return;
-  const int t = (int)(row / a.nq), h = (int)(row % a.nq);
-  if (a.cu_q != nullptr && (t < a.cu_q[0] || t >= a.cu_q[a.B])) return;  // a row behind the last sequence
-  const int NS = pl.slots();
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, NS = pl.slots();
+  const int t = (int)((uint32_t)row / (uint32_t)a.nq), h = (int)((uint32_t)row % (uint32_t)a.nq);
   const float* lse = pl.part_lse + row * NS;
   const float* po = pl.part_o + row * NS * HD;
+  nvb::pdl_wait();
+  nvb::pdl_trigger();
+  if (row >= (long)a.T * a.nq) return;
   float M = -INFINITY;
   for (int s = lane; s < NS; s += 32) M = fmaxf(M, lse[s]);
+  if (a.cu_q != nullptr && (t < a.cu_q[0] || t >= a.cu_q[a.B])) return;  // a row behind the last sequence
   M = nvb::warp_max(M);
   constexpr int PER = HD / 32;  // 2, 4 or 8 values per lane
   float acc[PER];
