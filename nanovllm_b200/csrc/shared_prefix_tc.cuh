@@ -489,9 +489,11 @@ __global__ void __launch_bounds__(384, 1) sp_tc_kernel(const __grid_constant__ C
         }
         const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
         if (__any_sync(0xffffffffu, top > 8.f)) {
-          // The maximum in use moves; O, l, the weights of the columns before and these ones follow.
-          const float f = top > 8.f ? exp2f(-top) : 1.f;
-          if (top > 8.f) m_used += top;
+          // The maximum in use moves; O, l, the weights of the columns before and these ones follow.  By a whole power of
+          // two, so that weights which have been rounded to bf16 are not rounded again.
+          const float up = top > 8.f ? ceilf(top) : 0.f;
+          const float f = up > 126.f ? 0.f : __int_as_float((127 - (int)up) << 23);
+          m_used += up;
           if (j > 0) rescale_o(f);
           l *= f;
           rs0 = fma2(rs0, pack2(f, f), 0), rs1 = fma2(rs1, pack2(f, f), 0);

@@ -168,6 +168,24 @@ def test_many_rows_masks_and_scales(window, softcap, amp, scale, batch, nq, nkv,
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("step", [3, 7, 32, 45, 128])
+@pytest.mark.parametrize("nq,nkv,hd", [(8, 2, 128), (4, 2, 64), (4, 1, 256)])
+def test_rising_scores(step, nq, nkv, hd, dev):
+    """Scores that grow by 6.5 (9.4 powers of two) every few keys while the values shrink as much, so that every key keeps
+    its share of the output through each move of the maximum."""
+    s = make(512, [40] * 40, [1, 3] * 20, nq, nkv, hd, seed=step, spare=0)
+    s["q"].zero_()[..., 0] = 1.0
+    s["q"][::3, :, 0] = 0.5
+    level = (torch.arange(512) // step).clamp(max=9).float()
+    for i, p in enumerate(s["prefix_blocks"].tolist()):
+        own = level[i * BS:(i + 1) * BS]
+        s["k_cache"][p] = 0.0
+        s["k_cache"][p, :, :, 0] = (6.5 * own).bfloat16()
+        s["v_cache"][p] = (s["v_cache"][p].float() * torch.exp(-6.5 * own)[None, :, None]).bfloat16()
+    check(call(s, dev, 1.0), s, 1.0)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_large_scores(dev):
     """Scores spread over tens of units: the running maximum moves from tile to tile."""
     s = make(700, [300, 10], [1, 3], 8, 2, 128, seed=9, amp=3.0)
